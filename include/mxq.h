@@ -400,7 +400,46 @@ int mxq_linear_fwd_static(const void* x, int x_dtype, int64_t M, int64_t K, int 
 int64_t mxq_linear_static_max_elems(void);
 int mxq_linear_static_status(void);
 
-/* Reads (and optionally clears) the current device's status word: 0, or
+/*
+ * 8-bit quantization with one fp32 scale per 128 values.  A block with maximum magnitude a has the scale
+ * s = max(a, 2^-100) * (1 / top), r = 1 / s and the codes RNE(v * r), in e4m3 (fmt 0, top 448) or e5m2 (fmt 1, top
+ * 57344); 1 / top, s, r and v * r are fp32, each rounded to nearest.  A block that holds an infinity or a NaN has that as its scale.
+ *   x         [rows, cols] of `dtype`, row_stride elements from row to row
+ *   codes     [rows, cols] bytes, codes_pitch (>= cols, % 16 == 0) bytes from row to row, 16-byte aligned; blocks along
+ *             cols; the bytes between cols rounded up to 8 and the pitch are not written.  NULL: not wanted
+ *   scales    [ceil(cols/128), rows]; with `tile` != 0 a block is 128 x 128 and scales is [ceil(cols/128), ceil(rows/128)]
+ *   codes_t   [cols, rows] bytes: the transposed operand, blocks along rows; its scales_t is [ceil(rows/128), cols], with
+ *             `tile` [ceil(rows/128), ceil(cols/128)].  NULL: not wanted (one of the two operands has to be)
+ *   colsum    [ceil(rows/128), cols] or NULL: fp32 sums of x over the rows of each row block, for mxq_sum_partials
+ */
+int mxq_fp8_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, int fmt, int tile,
+                     void* codes, int64_t codes_pitch, float* scales, void* codes_t, int64_t codes_t_pitch,
+                     float* scales_t, float* colsum, void* stream);
+
+/* out[c] = sum over i < n of part[i, c] (fp32, in a fixed order), rounded once to `dtype`. */
+int mxq_sum_partials(const float* part, int64_t n, int64_t cols, void* out, int dtype, void* stream);
+
+/*
+ * out[m, n] = sum over 128-blocks kb of K of sa[kb, m] * sb[kb, n] * (sum over k in kb of a[m, k] * b[n, k]) (+ bias[n]),
+ * rounded once to out_dtype.  a [M, K], b [N, K]: operands as mxq_fp8_quantize writes them (`*_fmt` 0 e4m3, 1 e5m2;
+ * `*_tile`: scales of 128 x 128 blocks); out [M, N] contiguous; bias [N] of bias_dtype, or NULL.  The product of two scales
+ * has to be representable in fp32.  Sums are fp32; results do not depend on timing.  K > 0.
+ */
+int mxq_fp8_gemm(const void* a, int64_t a_pitch, const float* a_scales, int a_tile, int a_fmt, const void* b,
+                 int64_t b_pitch, const float* b_scales, int b_tile, int b_fmt, void* out, int out_dtype,
+                 const void* bias, int bias_dtype, int64_t M, int64_t N, int64_t K, void* stream);
+
+/*
+ * y = x w^T (+ bias) with x [M, K] quantized in the call (1 x 128 blocks along K) and a weight that is packed already.
+ * The packed activations live in `workspace` (256-byte aligned, >= mxq_fp8_linear_workspace_bytes(M, K)).
+ */
+int64_t mxq_fp8_linear_workspace_bytes(int64_t M, int64_t K);
+int mxq_fp8_linear_fwd(const void* x, int x_dtype, int64_t x_stride, int x_fmt, const void* w, int64_t w_pitch,
+                       const float* w_scales, int w_tile, int w_fmt, void* y, int y_dtype, const void* bias,
+                       int bias_dtype, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
+                       void* stream);
+
+/* Reads (and optionally clears) the current device's status words: 0, or
  * MXQ_ERR_DEVICE after a kernel timed out on a wait.  The read is a blocking
  * cudaMemcpy, which does not wait for work on non-blocking streams:
  * synchronize the streams the GEMMs ran on first. */

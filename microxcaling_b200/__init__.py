@@ -20,3 +20,4 @@ from .simd_ops import simd_reduce_sum, simd_reduce_mean, simd_norm  # noqa: F401
 from .softmax import Softmax, softmax  # noqa: F401
 from .convolution import Conv1d, Conv2d, Conv3d, ConvTranspose2d, conv1d, conv2d, conv3d, conv_transpose2d  # noqa: F401
 from .rnn import LSTM  # noqa: F401
+from .fp8_block import BlockFP8, Fp8BlockLinear, fp8_block_linear, fp8_block_matmul, quantize_fp8_block  # noqa: F401

@@ -79,6 +79,12 @@ def lib():
         L.mxq_matmul_fwd.argtypes = [vp, vp, i32, i64, i64, i64, i64, i32, i32, fp, fp, i32, i32, vp, vp, vp, i32, i32, i32,
                                      vp, vp, i64, vp]
         L.mxq_gemm_sm_budget.argtypes = [i32]
+        L.mxq_fp8_quantize.argtypes = [vp, i32, i64, i64, i64, i32, i32, vp, i64, vp, vp, i64, vp, vp, vp]
+        L.mxq_sum_partials.argtypes = [vp, i64, i64, vp, i32, vp]
+        L.mxq_fp8_gemm.argtypes = [vp, i64, vp, i32, i32, vp, i64, vp, i32, i32, vp, i32, vp, i32, i64, i64, i64, vp]
+        L.mxq_fp8_linear_workspace_bytes.argtypes = [i64, i64]
+        L.mxq_fp8_linear_workspace_bytes.restype = i64
+        L.mxq_fp8_linear_fwd.argtypes = [vp, i32, i64, i32, vp, i64, vp, i32, i32, vp, i32, vp, i32, i64, i64, i64, vp, i64, vp]
         L.mxq_cpu_quantize_mx.argtypes = [vp, vp, i32, i64, i64, i64, i32, i32, i32, i32, f32, i32, i32, vp, i32]
         L.mxq_cpu_quantize_elemwise.argtypes = [vp, vp, i32, i32, i64, i32, i32, f32, i32, i32, i32, vp, i32]
         _lib = L
@@ -549,6 +555,73 @@ def rmsnorm_bf16(x, weight, bias, eps, want_saved=False):
         check(lib().mxq_rmsnorm_bf16(_ptr(x), _ptr(weight), _ptr(bias), _ptr(out), _ptr(xn), _ptr(ri), rows, hidden,
                                      float(eps), _stream(x)))
     return (out, xn, ri) if want_saved else out
+
+
+_F8 = (torch.float8_e4m3fn, torch.float8_e5m2)               # index = the library's format id
+
+
+def rows_of(t):
+    """t as [rows, last dimension] with unit stride inside a row (a view where the strides allow it)."""
+    t = t.reshape(-1, t.shape[-1]) if t.dim() != 2 else t
+    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
+
+
+def fp8_quantize(x, fmt, tile=False, rows=True, cols=False, colsum=False):
+    """8-bit codes and fp32 scales of a 2-D CUDA tensor, see mxq_fp8_quantize: (codes, scales), the same of the transposed
+    operand, column sums [row blocks, columns]; None for what is not asked for.  x: unit stride inside a row."""
+    R, C = x.shape
+    rb, cb = (R + 127) // 128, (C + 127) // 128
+    u8 = dict(dtype=torch.uint8, device=x.device)
+    f32 = dict(dtype=torch.float32, device=x.device)
+    pitch, pitch_t = (C + 15) // 16 * 16, (R + 15) // 16 * 16
+    codes = torch.empty((R, pitch), **u8) if rows else None
+    scales = torch.empty((cb, rb if tile else R), **f32) if rows else None
+    codes_t = torch.empty((C, pitch_t), **u8) if cols else None
+    scales_t = torch.empty((rb, cb if tile else C), **f32) if cols else None
+    sums = torch.empty((rb, C), **f32) if colsum else None
+    with _device_of(x.device):
+        check(lib().mxq_fp8_quantize(_ptr(x), _DT[x.dtype], R, C, x.stride(0) if R > 1 else C, fmt, int(tile), _ptr(codes), pitch,
+                                     _ptr(scales), _ptr(codes_t), pitch_t, _ptr(scales_t), _ptr(sums), _stream(x)))
+    a = (codes.view(_F8[fmt])[:, :C], scales) if rows else None
+    b = (codes_t.view(_F8[fmt])[:, :R], scales_t) if cols else None
+    return a, b, sums
+
+
+def sum_partials(part, dtype):
+    """part [n, columns] fp32 summed over n, rounded once to dtype."""
+    out = torch.empty(part.shape[1], dtype=dtype, device=part.device)
+    with _device_of(part.device):
+        check(lib().mxq_sum_partials(_ptr(part), part.shape[0], part.shape[1], _ptr(out), _DT[dtype], _stream(part)))
+    return out
+
+
+def _pitch(codes):
+    """Row pitch of an operand's codes; that of a single row is never used as an address, but has to be a legal one."""
+    return codes.stride(0) if codes.shape[0] > 1 else (codes.shape[1] + 15) // 16 * 16
+
+
+def fp8_gemm(a, b, bias, out_dtype):
+    """a b^T (+ bias) of two 8-bit block operands (fp8_block.BlockFP8); see mxq_fp8_gemm."""
+    (M, K), N = a.codes.shape, b.codes.shape[0]
+    out = torch.empty((M, N), dtype=out_dtype, device=a.codes.device)
+    with _device_of(out.device):
+        check(lib().mxq_fp8_gemm(_ptr(a.codes), _pitch(a.codes), _ptr(a.scales), int(a.tile), a.fmt, _ptr(b.codes),
+                                 _pitch(b.codes), _ptr(b.scales), int(b.tile), b.fmt, _ptr(out), _DT[out_dtype], _ptr(bias),
+                                 _DT[bias.dtype] if bias is not None else 0, M, N, K, _stream(out)))
+    return out
+
+
+def fp8_linear_fwd(x, x_fmt, w, bias):
+    """x w^T (+ bias), x [M, K] quantized in the call, w a fp8_block.BlockFP8; see mxq_fp8_linear_fwd."""
+    (M, K), N = x.shape, w.codes.shape[0]
+    L = lib()
+    ws = torch.empty(L.mxq_fp8_linear_workspace_bytes(M, K), dtype=torch.uint8, device=x.device)
+    y = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    with _device_of(x.device):
+        check(L.mxq_fp8_linear_fwd(_ptr(x), _DT[x.dtype], x.stride(0) if M > 1 else K, x_fmt, _ptr(w.codes), _pitch(w.codes),
+                                   _ptr(w.scales), int(w.tile), w.fmt, _ptr(y), _DT[y.dtype], _ptr(bias),
+                                   _DT[bias.dtype] if bias is not None else 0, M, N, K, _ptr(ws), ws.numel(), _stream(x)))
+    return y
 
 
 def launch_count(what):

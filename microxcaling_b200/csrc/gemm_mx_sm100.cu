@@ -27,6 +27,7 @@
 #include <algorithm>
 #include <cstring>
 #include <mutex>
+#include "fp8_block.cuh"
 #include "mxq_common.cuh"
 #include "sm100_ptx.cuh"
 #include "tma_host.cuh"
@@ -847,5 +848,6 @@ extern "C" int mxq_device_status(int clear) {
     int v = 0;
     if (cudaMemcpy(&v, w, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return MXQ_ERR_CUDA;
     if (clear && v != 0) cudaMemset(w, 0, sizeof(int));
-    return v;
+    const int f = mxq::fp8_gemm_status(clear);
+    return v != 0 ? v : f;
 }
