@@ -439,6 +439,38 @@ int mxq_fp8_linear_fwd(const void* x, int x_dtype, int64_t x_stride, int x_fmt, 
                        int bias_dtype, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
                        void* stream);
 
+/*
+ * Layer normalisation over the last dimension: y = (x - mean) / sqrt(var + eps) * w + b in fp32, rounded once.
+ *   x       [rows, cols] of dtype, x_stride elements from row to row; y [rows, cols] contiguous, of dtype
+ *   w, b    [cols] of w_dtype (dtype's or fp32), or NULL
+ *   mean, rstd  [rows] fp32, kept for the gradient; both or neither
+ * Gradient: dx [rows, cols] contiguous (NULL: not wanted) and partials [mxq_layer_norm_partials(rows, cols), 2, cols] fp32 (NULL: not wanted),
+ * whose sums over the first axis (mxq_sum_partials with 2 * cols columns) are dw and db.  rows == 0 writes nothing.
+ */
+int mxq_layer_norm_fwd(const void* x, int dtype, int64_t x_stride, const void* w, const void* b, int w_dtype, void* y,
+                       float* mean, float* rstd, int64_t rows, int64_t cols, float eps, void* stream);
+int64_t mxq_layer_norm_partials(int64_t rows, int64_t cols);
+int mxq_layer_norm_bwd(const void* dy, const void* x, int dtype, int64_t dy_stride, int64_t x_stride, const void* w,
+                       int w_dtype, const float* mean, const float* rstd, void* dx, float* partials, int64_t rows,
+                       int64_t cols, void* stream);
+
+/*
+ * Log probabilities of given tokens under softmax(logits * inv_temperature), entropies and the best alternatives.
+ *   logits     [rows, vocab] of dtype, stride elements from row to row
+ *   tokens     [rows] or NULL; ignore_index gives 0, any other index outside [0, vocab) gives NaN
+ *   logprobs   [rows] fp32 (with tokens); entropy, lse: [rows] fp32 or NULL (lse is what the gradient needs)
+ *   top        0 .. 32: the largest logits, largest first, the lowest index first among equals (NaN above all):
+ *              their log probabilities [rows, top] fp32 and indices [rows, top]
+ * A row with no logit above -inf has log probability -inf, entropy 0 and gradient 0.
+ * Gradient of sum(g_logprobs * logprobs) + sum(g_entropy * entropy): grad [rows, vocab] of dtype; either g may be NULL.
+ */
+int mxq_token_logprobs(const void* logits, int dtype, int64_t stride, const int64_t* tokens, int64_t ignore_index,
+                       float inv_temperature, float* logprobs, float* entropy, float* lse, int top, float* top_logprobs,
+                       int64_t* top_tokens, int64_t rows, int64_t vocab, void* stream);
+int mxq_token_logprobs_grad(const void* logits, int dtype, int64_t stride, const int64_t* tokens, int64_t ignore_index,
+                            float inv_temperature, const float* lse, const float* entropy, const float* g_logprobs,
+                            const float* g_entropy, void* grad, int64_t rows, int64_t vocab, void* stream);
+
 /* Reads (and optionally clears) the current device's status words: 0, or
  * MXQ_ERR_DEVICE after a kernel timed out on a wait.  The read is a blocking
  * cudaMemcpy, which does not wait for work on non-blocking streams:

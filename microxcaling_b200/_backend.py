@@ -81,6 +81,12 @@ def lib():
         L.mxq_gemm_sm_budget.argtypes = [i32]
         L.mxq_fp8_quantize.argtypes = [vp, i32, i64, i64, i64, i32, i32, vp, i64, vp, vp, i64, vp, vp, vp]
         L.mxq_sum_partials.argtypes = [vp, i64, i64, vp, i32, vp]
+        L.mxq_layer_norm_fwd.argtypes = [vp, i32, i64, vp, vp, i32, vp, vp, vp, i64, i64, f32, vp]
+        L.mxq_layer_norm_partials.argtypes = [i64, i64]
+        L.mxq_layer_norm_partials.restype = i64
+        L.mxq_layer_norm_bwd.argtypes = [vp, vp, i32, i64, i64, vp, i32, vp, vp, vp, vp, i64, i64, vp]
+        L.mxq_token_logprobs.argtypes = [vp, i32, i64, vp, i64, f32, vp, vp, vp, i32, vp, vp, i64, i64, vp]
+        L.mxq_token_logprobs_grad.argtypes = [vp, i32, i64, vp, i64, f32, vp, vp, vp, vp, vp, i64, i64, vp]
         L.mxq_fp8_gemm.argtypes = [vp, i64, vp, i32, i32, vp, i64, vp, i32, i32, vp, i32, vp, i32, i64, i64, i64, vp]
         L.mxq_fp8_linear_workspace_bytes.argtypes = [i64, i64]
         L.mxq_fp8_linear_workspace_bytes.restype = i64
@@ -622,6 +628,65 @@ def fp8_linear_fwd(x, x_fmt, w, bias):
                                    _ptr(w.scales), int(w.tile), w.fmt, _ptr(y), _DT[y.dtype], _ptr(bias),
                                    _DT[bias.dtype] if bias is not None else 0, M, N, K, _ptr(ws), ws.numel(), _stream(x)))
     return y
+
+
+def layer_norm_fwd(x, weight, bias, eps, want_saved):
+    """(y, mean, rstd) of x [rows, cols] (unit stride inside a row); mean and rstd are None unless wanted; see mxq_layer_norm_fwd."""
+    rows, cols = x.shape
+    y = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
+    mean = rstd = None
+    if want_saved:
+        mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+    w = weight if weight is not None else bias
+    with _device_of(x.device):
+        check(lib().mxq_layer_norm_fwd(_ptr(x), _DT[x.dtype], x.stride(0) if rows > 1 else cols, _ptr(weight), _ptr(bias),
+                                       _DT[x.dtype if w is None else w.dtype], _ptr(y), _ptr(mean), _ptr(rstd), rows, cols, eps,
+                                       _stream(x)))
+    return y, mean, rstd
+
+
+def layer_norm_bwd(dy, x, weight, mean, rstd, want_dx, want_sums):
+    """(dx or None, partial sums of dw and db [CTAs, 2 * cols] or None); see mxq_layer_norm_bwd."""
+    rows, cols = x.shape
+    dx = torch.empty((rows, cols), dtype=x.dtype, device=x.device) if want_dx else None
+    L = lib()
+    with _device_of(x.device):
+        part = torch.empty((L.mxq_layer_norm_partials(rows, cols), 2 * cols), dtype=torch.float32, device=x.device) \
+            if want_sums else None
+        check(L.mxq_layer_norm_bwd(_ptr(dy), _ptr(x), _DT[x.dtype], dy.stride(0) if rows > 1 else cols,
+                                   x.stride(0) if rows > 1 else cols, _ptr(weight),
+                                   _DT[x.dtype if weight is None else weight.dtype], _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(part),
+                                   rows, cols, _stream(x)))
+    return dx, part
+
+
+LOGPROBS_MAX_TOP = 32
+
+
+def token_logprobs(x, tokens, ignore_index, inv_t, entropy, top, want_lse):
+    """(logprobs, entropy, lse, top logprobs, top tokens) of x [rows, vocab]; None for what is not wanted; see mxq_token_logprobs."""
+    rows, vocab = x.shape
+    f32 = dict(dtype=torch.float32, device=x.device)
+    lp = torch.empty(rows, **f32) if tokens is not None else None
+    h = torch.empty(rows, **f32) if entropy else None
+    lse = torch.empty(rows, **f32) if want_lse else None
+    tlp = torch.empty((rows, top), **f32) if top else None
+    tok = torch.empty((rows, top), dtype=torch.int64, device=x.device) if top else None
+    with _device_of(x.device):
+        check(lib().mxq_token_logprobs(_ptr(x), _DT[x.dtype], x.stride(0) if rows > 1 else vocab, _ptr(tokens), ignore_index, inv_t,
+                                       _ptr(lp), _ptr(h), _ptr(lse), top, _ptr(tlp), _ptr(tok), rows, vocab, _stream(x)))
+    return lp, h, lse, tlp, tok
+
+
+def token_logprobs_grad(x, tokens, ignore_index, inv_t, lse, entropy, g_lp, g_h):
+    """Gradient [rows, vocab] with respect to x; see mxq_token_logprobs_grad."""
+    rows, vocab = x.shape
+    dx = torch.empty((rows, vocab), dtype=x.dtype, device=x.device)
+    with _device_of(x.device):
+        check(lib().mxq_token_logprobs_grad(_ptr(x), _DT[x.dtype], x.stride(0) if rows > 1 else vocab, _ptr(tokens), ignore_index,
+                                            inv_t, _ptr(lse), _ptr(entropy), _ptr(g_lp), _ptr(g_h), _ptr(dx), rows, vocab,
+                                            _stream(x)))
+    return dx
 
 
 def launch_count(what):

@@ -1,0 +1,411 @@
+// Layer normalisation over the last dimension, forward and backward, each value rounded once (sm_100a).
+//
+//     y = (x - mean) * rstd * w + b,   rstd = 1 / sqrt(var + eps)
+//     with g = dy * w and n = (x - mean) * rstd:   dx = rstd * (g - mean(g) - n * mean(g * n)),
+//     dw = sum over rows of dy * n,   db = sum over rows of dy
+//
+// Bound by HBM: forward reads x and writes y, backward reads x and dy and writes dx.  A row stays in the registers of
+// one group of threads (a warp for short rows, a CTA for long ones) between its statistics and its use; the variance is that of the
+// centred values, not a difference of two sums.  Backward CTAs walk the rows with a stride and keep the sums for dw and db of
+// "their" rows in fp32 registers, column by column (each thread owns the same columns of every row), and write
+// them once: [CTA, 2, cols] partial sums, which mxq_sum_partials adds in a fixed order.  Rows longer than the
+// registers hold are read twice (the second time from L2) and their column sums are kept in shared memory, or, longer
+// still, in the workspace itself.
+#include <algorithm>
+#include "fp8_block.cuh"
+#include "mxq_common.cuh"
+
+namespace mxq {
+
+struct NormArgs {
+    const void* x;
+    const void* dy;              // backward
+    const void* w;               // [cols] or null
+    const void* b;               // [cols] or null (forward)
+    void* out;                   // y or dx (backward: or null)
+    float* mean;                 // [rows], forward: or null
+    float* rstd;
+    float* part;                 // backward: [CTAs, 2, cols] or null
+    int64_t rows, cols, x_stride, dy_stride;
+    float eps;
+};
+
+// VEC consecutive values as fp32
+template <int DT, int VEC>
+__device__ __forceinline__ void load_vec(const void* base, int64_t i, float (&v)[VEC]) {
+    if constexpr (VEC == 1) {
+        v[0] = load1<DT>(base, i);
+    } else {
+        constexpr int N = VecIO<DT, 16>::N;
+#pragma unroll
+        for (int j = 0; j < VEC; j += N) {
+            uint32_t b[N];
+            VecIO<DT, 16>::load(base, i + j, b);
+#pragma unroll
+            for (int k = 0; k < N; ++k) v[j + k] = __uint_as_float(b[k]);
+        }
+    }
+}
+template <int DT, int VEC>
+__device__ __forceinline__ void store_vec(void* base, int64_t i, const float (&v)[VEC]) {
+    if constexpr (VEC == 1) {
+        store1<DT>(base, i, v[0]);
+    } else if constexpr (DT == DT_F32) {
+        float4* p = reinterpret_cast<float4*>(reinterpret_cast<float*>(base) + i);
+#pragma unroll
+        for (int j = 0; j < VEC; j += 4) p[j / 4] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+    } else {
+        uint32_t w[VEC / 2];
+#pragma unroll
+        for (int j = 0; j < VEC / 2; ++j) {
+            if constexpr (DT == DT_BF16) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+                w[j] = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+                const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+                w[j] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+        }
+        static_assert(VEC == 8, "one 16-byte store");
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(base) + i) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+// Sums of a and b over the TPR threads of a row, in every one of them.  Groups longer than a warp are the whole CTA;
+// `buf` alternates between two halves of `red`, so one barrier a call is enough.
+template <int TPR>
+__device__ __forceinline__ void row_sum2(float& a, float& b, float2 (*red)[32], int buf) {
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) {
+        a += __shfl_xor_sync(0xffffffffu, a, s);
+        b += __shfl_xor_sync(0xffffffffu, b, s);
+    }
+    if constexpr (TPR > 32) {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        if (lane == 0) red[buf][warp] = make_float2(a, b);
+        __syncthreads();
+        const float2 t = lane < TPR / 32 ? red[buf][lane] : make_float2(0.f, 0.f);
+        a = t.x; b = t.y;
+#pragma unroll
+        for (int s = TPR / 64; s > 0; s >>= 1) {
+            a += __shfl_xor_sync(0xffffffffu, a, s);
+            b += __shfl_xor_sync(0xffffffffu, b, s);
+        }
+        a = __shfl_sync(0xffffffffu, a, 0);
+        b = __shfl_sync(0xffffffffu, b, 0);
+    }
+}
+
+// threads of a CTA: eight rows of a warp each, or one row
+template <int TPR> constexpr int kNormThreads = TPR == 32 ? 256 : TPR;
+
+// A row in registers: thread t of the row's TPR threads owns the NV groups of VEC columns at (i * TPR + t) * VEC.
+template <int DT, int WDT, int VEC, int TPR, int NV>
+__global__ void __launch_bounds__(kNormThreads<TPR>) layer_norm_fwd_kernel(const NormArgs g) {
+    __shared__ float2 red[2][32];
+    const int t = threadIdx.x % TPR;
+    const int64_t row = (int64_t)blockIdx.x * (kNormThreads<TPR> / TPR) + threadIdx.x / TPR;
+    if (TPR == 32 && row >= g.rows) return;                    // a warp on its own; a CTA-wide row always exists
+    using T = typename Store<DT>::T;
+    const T* x = reinterpret_cast<const T*>(g.x) + row * g.x_stride;
+    float v[NV][VEC];
+    float s = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int64_t c = (int64_t)(i * TPR + t) * VEC;
+        if (c < g.cols) load_vec<DT, VEC>(x, c, v[i]);
+        else
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[i][j] = 0.f;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) s += v[i][j];
+    }
+    row_sum2<TPR>(s, s2, red, 0);
+    const float mean = s / (float)g.cols;
+    s = s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if ((int64_t)(i * TPR + t) * VEC < g.cols) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) { v[i][j] -= mean; s = __fmaf_rn(v[i][j], v[i][j], s); }
+        }
+    }
+    row_sum2<TPR>(s, s2, red, 1);
+    const float rstd = 1.f / sqrtf(s / (float)g.cols + g.eps);
+    if (t == 0 && g.mean) { g.mean[row] = mean; g.rstd[row] = rstd; }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int64_t c = (int64_t)(i * TPR + t) * VEC;
+        if (c >= g.cols) continue;
+        float w[VEC], b[VEC];
+        if (g.w) load_vec<WDT, VEC>(g.w, c, w);
+        if (g.b) load_vec<WDT, VEC>(g.b, c, b);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            float n = v[i][j] * rstd;
+            if (g.w) n *= w[j];
+            if (g.b) n += b[j];
+            v[i][j] = n;
+        }
+        store_vec<DT, VEC>(g.out, row * g.cols + c, v[i]);
+    }
+}
+
+// Rows of any length: read three times, the later ones from L2.
+template <int DT, int WDT>
+__global__ void __launch_bounds__(1024) layer_norm_fwd_long_kernel(const NormArgs g) {
+    __shared__ float2 red[2][32];
+    const int64_t row = blockIdx.x;
+    using T = typename Store<DT>::T;
+    const T* x = reinterpret_cast<const T*>(g.x) + row * g.x_stride;
+    float s = 0.f, z = 0.f;
+    for (int64_t c = threadIdx.x; c < g.cols; c += 1024) s += load1<DT>(x, c);
+    row_sum2<1024>(s, z, red, 0);
+    const float mean = s / (float)g.cols;
+    s = z = 0.f;
+    for (int64_t c = threadIdx.x; c < g.cols; c += 1024) { const float d = load1<DT>(x, c) - mean; s = __fmaf_rn(d, d, s); }
+    row_sum2<1024>(s, z, red, 1);
+    const float rstd = 1.f / sqrtf(s / (float)g.cols + g.eps);
+    if (threadIdx.x == 0 && g.mean) { g.mean[row] = mean; g.rstd[row] = rstd; }
+    for (int64_t c = threadIdx.x; c < g.cols; c += 1024) {
+        float n = (load1<DT>(x, c) - mean) * rstd;
+        if (g.w) n *= load1<WDT>(g.w, c);
+        if (g.b) n += load1<WDT>(g.b, c);
+        store1<DT>(g.out, row * g.cols + c, n);
+    }
+}
+
+template <int DT, int WDT, int VEC, int TPR, int NV>
+__global__ void __launch_bounds__(kNormThreads<TPR>) layer_norm_bwd_kernel(const NormArgs g) {
+    constexpr int ROWS = kNormThreads<TPR> / TPR;
+    __shared__ float2 red[2][32];
+    const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
+    using T = typename Store<DT>::T;
+    float dw[NV][VEC], db[NV][VEC];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) dw[i][j] = db[i][j] = 0.f;
+    const float inv = 1.f / (float)g.cols;
+    int buf = 0;
+    for (int64_t row = (int64_t)blockIdx.x * ROWS + group; row < g.rows; row += (int64_t)gridDim.x * ROWS, buf ^= 1) {
+        const T* x = reinterpret_cast<const T*>(g.x) + row * g.x_stride;
+        const T* dy = reinterpret_cast<const T*>(g.dy) + row * g.dy_stride;
+        const float mean = g.mean[row], rstd = g.rstd[row];
+        float n[NV][VEC], d[NV][VEC];
+        float s = 0.f, sn = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int64_t c = (int64_t)(i * TPR + t) * VEC;
+            if (c < g.cols) {
+                load_vec<DT, VEC>(x, c, n[i]);
+                load_vec<DT, VEC>(dy, c, d[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int64_t c = (int64_t)(i * TPR + t) * VEC;
+            if (c >= g.cols) continue;
+            float w[VEC];
+            if (g.w) load_vec<WDT, VEC>(g.w, c, w);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                n[i][j] = (n[i][j] - mean) * rstd;
+                dw[i][j] = __fmaf_rn(d[i][j], n[i][j], dw[i][j]);
+                db[i][j] += d[i][j];
+                if (g.w) d[i][j] *= w[j];
+                s += d[i][j];
+                sn = __fmaf_rn(d[i][j], n[i][j], sn);
+            }
+        }
+        if (!g.out) continue;                                  // the same for every thread
+        row_sum2<TPR>(s, sn, red, buf);
+        s *= inv; sn *= inv;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int64_t c = (int64_t)(i * TPR + t) * VEC;
+            if (c >= g.cols) continue;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) d[i][j] = rstd * (d[i][j] - s - n[i][j] * sn);
+            store_vec<DT, VEC>(g.out, row * g.cols + c, d[i]);
+        }
+    }
+    if (!g.part) return;
+    float* part = g.part + (int64_t)blockIdx.x * 2 * g.cols;
+    if constexpr (ROWS == 1) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int64_t c = (int64_t)(i * TPR + t) * VEC;
+            if (c >= g.cols) continue;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) { part[c + j] = dw[i][j]; part[g.cols + c + j] = db[i][j]; }
+        }
+    } else {
+        // the CTA's warps add their sums one after the other
+        __shared__ float acc[2][TPR * NV * VEC];
+        for (int r = 0; r < ROWS; ++r) {
+            if (group == r) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) {
+                        const int c = (i * TPR + t) * VEC + j;
+                        acc[0][c] = r ? acc[0][c] + dw[i][j] : dw[i][j];
+                        acc[1][c] = r ? acc[1][c] + db[i][j] : db[i][j];
+                    }
+            }
+            __syncthreads();
+        }
+        for (int c = threadIdx.x; c < g.cols; c += kNormThreads<TPR>) { part[c] = acc[0][c]; part[g.cols + c] = acc[1][c]; }
+    }
+}
+
+// Rows of any length: read twice; column sums in shared memory (SMEM) or in this CTA's rows of the workspace.
+template <int DT, int WDT, bool SMEM>
+__global__ void __launch_bounds__(1024) layer_norm_bwd_long_kernel(const NormArgs g) {
+    extern __shared__ float sums[];
+    __shared__ float2 red[2][32];
+    using T = typename Store<DT>::T;
+    float* part = g.part ? g.part + (int64_t)blockIdx.x * 2 * g.cols : nullptr;
+    float* aw = SMEM ? sums : part;
+    float* ab = aw ? aw + g.cols : nullptr;
+    const bool keep = g.part != nullptr;
+    if (keep)
+        for (int64_t c = threadIdx.x; c < g.cols; c += 1024) aw[c] = ab[c] = 0.f;
+    const float inv = 1.f / (float)g.cols;
+    int buf = 0;
+    for (int64_t row = blockIdx.x; row < g.rows; row += gridDim.x, buf ^= 1) {
+        const T* x = reinterpret_cast<const T*>(g.x) + row * g.x_stride;
+        const T* dy = reinterpret_cast<const T*>(g.dy) + row * g.dy_stride;
+        const float mean = g.mean[row], rstd = g.rstd[row];
+        float s = 0.f, sn = 0.f;
+        for (int64_t c = threadIdx.x; c < g.cols; c += 1024) {
+            const float n = (load1<DT>(x, c) - mean) * rstd, d = load1<DT>(dy, c);
+            if (keep) { aw[c] = __fmaf_rn(d, n, aw[c]); ab[c] += d; }
+            const float h = g.w ? d * load1<WDT>(g.w, c) : d;
+            s += h;
+            sn = __fmaf_rn(h, n, sn);
+        }
+        if (!g.out) continue;
+        row_sum2<1024>(s, sn, red, buf);
+        s *= inv; sn *= inv;
+        for (int64_t c = threadIdx.x; c < g.cols; c += 1024) {
+            const float n = (load1<DT>(x, c) - mean) * rstd, d = load1<DT>(dy, c);
+            const float h = g.w ? d * load1<WDT>(g.w, c) : d;
+            store1<DT>(g.out, row * g.cols + c, rstd * (h - s - n * sn));
+        }
+    }
+    if (SMEM && keep)
+        for (int64_t c = threadIdx.x; c < g.cols; c += 1024) { part[c] = aw[c]; part[g.cols + c] = ab[c]; }   // a thread's own columns
+}
+
+// Threads a row and values a thread: the smallest group that holds the row at 16 values a thread (8 for a warp's
+// shortest rows), so that registers leave room for several CTAs on an SM.
+struct NormShape { int tpr, vals; };
+static NormShape norm_shape(int64_t cols) {
+    if (cols <= 256) return {32, 8};
+    if (cols <= 512) return {32, 16};
+    if (cols <= 1024) return {128, 8};
+    if (cols <= 2048) return {128, 16};
+    if (cols <= 4096) return {256, 16};
+    if (cols <= 8192) return {512, 16};
+    return {0, 0};
+}
+
+static int64_t norm_bwd_ctas(int64_t rows, int64_t cols) {
+    const NormShape s = norm_shape(cols);
+    const int64_t per = s.tpr == 32 ? 8 : 1, resident = s.tpr == 0 ? 1 : s.tpr >= 512 ? 1 : s.tpr >= 256 ? 2 : 4;
+    return std::max<int64_t>(1, std::min<int64_t>((rows + per - 1) / per, sm_count() * resident));
+}
+
+template <int DT, int WDT, int VEC, int TPR, int VALS>
+static int launch_norm(const NormArgs& g, bool bwd, cudaStream_t st) {
+    constexpr int threads = kNormThreads<TPR>;
+    if (bwd) {
+        layer_norm_bwd_kernel<DT, WDT, VEC, TPR, VALS / VEC><<<(int)norm_bwd_ctas(g.rows, g.cols), threads, 0, st>>>(g);
+    } else {
+        const int64_t grid = (g.rows + threads / TPR - 1) / (threads / TPR);
+        if (grid > 0x7fffffff) return MXQ_ERR_TOO_LARGE;
+        layer_norm_fwd_kernel<DT, WDT, VEC, TPR, VALS / VEC><<<(int)grid, threads, 0, st>>>(g);
+    }
+    return check_launch();
+}
+
+template <int DT, int WDT, int VEC>
+static int launch_norm_vec(const NormArgs& g, bool bwd, cudaStream_t st) {
+    const NormShape s = norm_shape(g.cols);
+    if (s.tpr == 32 && s.vals == 8) return launch_norm<DT, WDT, VEC, 32, 8>(g, bwd, st);
+    if (s.tpr == 32) return launch_norm<DT, WDT, VEC, 32, 16>(g, bwd, st);
+    if (s.tpr == 128 && s.vals == 8) return launch_norm<DT, WDT, VEC, 128, 8>(g, bwd, st);
+    if (s.tpr == 128) return launch_norm<DT, WDT, VEC, 128, 16>(g, bwd, st);
+    if (s.tpr == 256) return launch_norm<DT, WDT, VEC, 256, 16>(g, bwd, st);
+    return launch_norm<DT, WDT, VEC, 512, 16>(g, bwd, st);
+}
+
+template <int DT, int WDT>
+static int launch_norm_dt(const NormArgs& g, bool bwd, cudaStream_t st) {
+    if (norm_shape(g.cols).tpr) {
+        constexpr int VEC = DT == DT_F32 ? 4 : 8;
+        const int es = DT == DT_F32 ? 4 : 2;
+        // 16-byte accesses: whole vectors in a row, aligned rows, aligned weights
+        const bool vec = g.cols % VEC == 0 && aligned16(g.x) && aligned16(g.out) && g.x_stride * es % 16 == 0 &&
+                         aligned16(g.w) && aligned16(g.b) && (!bwd || (aligned16(g.dy) && g.dy_stride * es % 16 == 0));
+        return vec ? launch_norm_vec<DT, WDT, VEC>(g, bwd, st) : launch_norm_vec<DT, WDT, 1>(g, bwd, st);
+    }
+    if (!bwd) {
+        if (g.rows > 0x7fffffff) return MXQ_ERR_TOO_LARGE;
+        layer_norm_fwd_long_kernel<DT, WDT><<<(int)g.rows, 1024, 0, st>>>(g);
+        return check_launch();
+    }
+    const int grid = (int)norm_bwd_ctas(g.rows, g.cols);
+    const int64_t bytes = g.part ? 8 * g.cols : 0;
+    if (bytes <= 200 * 1024) {
+        auto kern = layer_norm_bwd_long_kernel<DT, WDT, true>;
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess) { cudaGetLastError(); return MXQ_ERR_CUDA; }
+        kern<<<grid, 1024, (size_t)bytes, st>>>(g);
+    } else {
+        layer_norm_bwd_long_kernel<DT, WDT, false><<<grid, 1024, 0, st>>>(g);
+    }
+    return check_launch();
+}
+
+static int norm_dispatch(const NormArgs& g, int dtype, int wdtype, bool bwd, cudaStream_t st) {
+    if (dtype == MXQ_F32) return wdtype == MXQ_F32 ? launch_norm_dt<DT_F32, DT_F32>(g, bwd, st) : MXQ_ERR_UNSUPPORTED;
+    if (dtype == MXQ_F16) {
+        if (wdtype == MXQ_F16) return launch_norm_dt<DT_F16, DT_F16>(g, bwd, st);
+        return wdtype == MXQ_F32 ? launch_norm_dt<DT_F16, DT_F32>(g, bwd, st) : MXQ_ERR_UNSUPPORTED;
+    }
+    if (wdtype == MXQ_BF16) return launch_norm_dt<DT_BF16, DT_BF16>(g, bwd, st);
+    return wdtype == MXQ_F32 ? launch_norm_dt<DT_BF16, DT_F32>(g, bwd, st) : MXQ_ERR_UNSUPPORTED;
+}
+
+}  // namespace mxq
+
+extern "C" int mxq_layer_norm_fwd(const void* x, int dtype, int64_t x_stride, const void* w, const void* b, int w_dtype, void* y,
+                                  float* mean, float* rstd, int64_t rows, int64_t cols, float eps, void* stream) {
+    using namespace mxq;
+    if (rows < 0 || cols <= 0 || dtype < 0 || dtype > 2 || w_dtype < 0 || w_dtype > 2 || !mean != !rstd) return MXQ_ERR_BAD_ARG;
+    if (rows == 0) return MXQ_OK;
+    if (!x || !y || (rows > 1 && x_stride < cols)) return MXQ_ERR_BAD_ARG;
+    NormArgs g = {};
+    g.x = x; g.w = w; g.b = b; g.out = y; g.mean = mean; g.rstd = rstd;
+    g.rows = rows; g.cols = cols; g.x_stride = x_stride; g.eps = eps;
+    return norm_dispatch(g, dtype, w_dtype, false, (cudaStream_t)stream);
+}
+
+extern "C" int64_t mxq_layer_norm_partials(int64_t rows, int64_t cols) {
+    return rows <= 0 || cols <= 0 ? 0 : mxq::norm_bwd_ctas(rows, cols);
+}
+
+extern "C" int mxq_layer_norm_bwd(const void* dy, const void* x, int dtype, int64_t dy_stride, int64_t x_stride, const void* w, int w_dtype,
+                                  const float* mean, const float* rstd, void* dx, float* partials, int64_t rows, int64_t cols,
+                                  void* stream) {
+    using namespace mxq;
+    if (rows < 0 || cols <= 0 || dtype < 0 || dtype > 2 || w_dtype < 0 || w_dtype > 2) return MXQ_ERR_BAD_ARG;
+    if (rows == 0 || (!dx && !partials)) return MXQ_OK;
+    if (!x || !dy || !mean || !rstd || (rows > 1 && (x_stride < cols || dy_stride < cols))) return MXQ_ERR_BAD_ARG;
+    NormArgs g = {};
+    g.x = x; g.dy = dy; g.w = w; g.out = dx; g.mean = const_cast<float*>(mean); g.rstd = const_cast<float*>(rstd); g.part = partials;
+    g.rows = rows; g.cols = cols; g.x_stride = x_stride; g.dy_stride = dy_stride;
+    return norm_dispatch(g, dtype, w_dtype, true, (cudaStream_t)stream);
+}

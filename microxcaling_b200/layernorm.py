@@ -1,8 +1,11 @@
 """bfloat-emulated RMSNorm (reference: mx/layernorm.py:98-200, fused kernel for bfloat16 CUDA tensors) and
-LayerNorm (mx/layernorm.py:17-96, 203-210)."""
+LayerNorm (mx/layernorm.py:17-96, 203-210).  fused_layer_norm / FusedLayerNorm have no counterpart there: a layer norm that
+emulates no vector format, computed in fp32 in one pass each way and rounded once."""
 import torch
+from torch.autograd.function import once_differentiable
 
 from ._autograd import call
+from ._backend import MxqError
 from .norm_utils import norm_backward_ln, norm_forward
 from .specs import apply_mx_specs, get_backwards_mx_specs, mx_assert_test
 from .vector_ops import (fused_bf16_ok, vec_add, vec_mul, vec_quantize, vec_recip, vec_reduce_mean, vec_reduce_sum,
@@ -121,3 +124,67 @@ def layer_norm(input, normalized_shape, weight, bias, eps=1e-12, mx_specs=None, 
         return torch_layer_norm(input, normalized_shape, weight, bias, eps)
     assert normalized_shape == weight.shape
     return LayerNormFunction.apply(input, weight, bias, eps, apply_mx_specs(mx_specs), name)
+
+
+class FusedLayerNormFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        from . import _backend
+        x2 = _backend.rows_of(x)
+        want = any(ctx.needs_input_grad[:3])
+        y, mean, rstd = _backend.layer_norm_fwd(x2, weight, bias, eps, want)
+        if want:
+            ctx.save_for_backward(x2, weight, mean, rstd)
+            ctx.bias_dtype = None if bias is None else bias.dtype
+        return y.view(x.shape)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        from . import _backend
+        x2, weight, mean, rstd = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dx, part = _backend.layer_norm_bwd(_backend.rows_of(dy), x2, weight, mean, rstd, need_x, need_w or need_b)
+        dw = db = None
+        if part is not None:
+            sums = _backend.sum_partials(part, weight.dtype if weight is not None else ctx.bias_dtype)
+            cols = x2.shape[1]
+            dw, db = sums[:cols] if need_w else None, sums[cols:] if need_b else None
+        return dx.view(dy.shape) if need_x else None, dw, db, None
+
+
+def fused_layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension, in fp32 and rounded once to x's dtype; no
+    vector format is emulated (layer_norm does that).  weight and bias: [cols], both of x's dtype or both float32; either may be
+    None.  Gradients: dx of x's dtype; dw and db summed over the rows in fp32, in a fixed order."""
+    if not isinstance(x, torch.Tensor) or x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise MxqError("x must be a float32, float16 or bfloat16 tensor")
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise MxqError("x needs at least one value along its last dimension")
+    if not eps >= 0:
+        raise MxqError("eps must not be negative")
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is not None and (t.shape != x.shape[-1:] or t.dtype not in (x.dtype, torch.float32) or t.device != x.device or
+                              not t.is_contiguous()):
+            raise MxqError("%s must be a contiguous tensor of %d values of x's dtype or float32 on x's device" % (name, x.shape[-1]))
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise MxqError("weight and bias must have one dtype")
+    if x.is_cuda:
+        return call(FusedLayerNormFunction, x, weight, bias, float(eps))
+    v = x.float()
+    d = v - v.mean(-1, keepdim=True)
+    y = d / ((d * d).mean(-1, keepdim=True) + eps).sqrt()
+    y = y if weight is None else y * weight.float()
+    return (y if bias is None else y + bias.float()).to(x.dtype)
+
+
+class FusedLayerNorm(torch.nn.LayerNorm):
+    """Layer normalisation over the last dimension on fused_layer_norm."""
+
+    def __init__(self, hidden_size, eps=1e-5, elementwise_affine=True, bias=True, device=None, dtype=None):
+        super().__init__(hidden_size, eps=eps, elementwise_affine=elementwise_affine, bias=bias, device=device, dtype=dtype)
+        if len(self.normalized_shape) != 1:
+            raise MxqError("FusedLayerNorm normalises the last dimension only")
+
+    def forward(self, x):
+        return fused_layer_norm(x, self.weight, self.bias, self.eps)
