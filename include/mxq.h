@@ -440,19 +440,37 @@ int mxq_fp8_linear_fwd(const void* x, int x_dtype, int64_t x_stride, int x_fmt, 
                        void* stream);
 
 /*
+ * The same layer in training, one call each way.  Forward quantizes x (1 x 128 blocks) and w (128 x 128 blocks), both to
+ * `fmt`, and multiplies; `saved` (mxq_fp8_linear_saved_bytes; need_dx, need_dw: which gradients will be wanted) keeps the transposed
+ * operands.  Backward quantizes dy to grad_fmt, once along N for dx [M, K] and once along M for dw [N, K], and sums it
+ * for db [N]; dx, dw and db may be NULL, saved_dx and saved_dw repeat forward's need_dx and need_dw.  saved and scratch
+ * (mxq_fp8_linear_scratch_bytes) are 256-byte aligned.  M, N, K > 0.
+ */
+int64_t mxq_fp8_linear_saved_bytes(int64_t M, int64_t N, int64_t K, int need_dx, int need_dw);
+int64_t mxq_fp8_linear_scratch_bytes(int64_t M, int64_t N, int64_t K, int backward);
+int mxq_fp8_linear_fwd_train(const void* x, int x_dtype, int64_t x_stride, const void* w, int w_dtype, int64_t w_stride,
+                             int fmt, const void* bias, int bias_dtype, void* y, int y_dtype, int need_dx, int need_dw,
+                             void* saved, int64_t saved_bytes, void* scratch, int64_t scratch_bytes, int64_t M,
+                             int64_t N, int64_t K, void* stream);
+int mxq_fp8_linear_bwd(const void* dy, int dy_dtype, int64_t dy_stride, int grad_fmt, int fmt, const void* saved,
+                       int64_t saved_bytes, int saved_dx, int saved_dw, void* dx, int dx_dtype, void* dw, int dw_dtype,
+                       void* db, int db_dtype, void* scratch, int64_t scratch_bytes, int64_t M, int64_t N, int64_t K,
+                       void* stream);
+
+/*
  * Layer normalisation over the last dimension: y = (x - mean) / sqrt(var + eps) * w + b in fp32, rounded once.
  *   x       [rows, cols] of dtype, x_stride elements from row to row; y [rows, cols] contiguous, of dtype
  *   w, b    [cols] of w_dtype (dtype's or fp32), or NULL
  *   mean, rstd  [rows] fp32, kept for the gradient; both or neither
- * Gradient: dx [rows, cols] contiguous (NULL: not wanted) and partials [mxq_layer_norm_partials(rows, cols), 2, cols] fp32 (NULL: not wanted),
- * whose sums over the first axis (mxq_sum_partials with 2 * cols columns) are dw and db.  rows == 0 writes nothing.
+ * Gradient: dx [rows, cols] contiguous, dw and db [cols] of sums_dtype (zeros for rows == 0); each may be NULL.  dw and db need a
+ * workspace of mxq_layer_norm_workspace_bytes(rows, cols) on the current device, 16-byte aligned.
  */
 int mxq_layer_norm_fwd(const void* x, int dtype, int64_t x_stride, const void* w, const void* b, int w_dtype, void* y,
                        float* mean, float* rstd, int64_t rows, int64_t cols, float eps, void* stream);
-int64_t mxq_layer_norm_partials(int64_t rows, int64_t cols);
+int64_t mxq_layer_norm_workspace_bytes(int64_t rows, int64_t cols);
 int mxq_layer_norm_bwd(const void* dy, const void* x, int dtype, int64_t dy_stride, int64_t x_stride, const void* w,
-                       int w_dtype, const float* mean, const float* rstd, void* dx, float* partials, int64_t rows,
-                       int64_t cols, void* stream);
+                       int w_dtype, const float* mean, const float* rstd, void* dx, void* dw, void* db, int sums_dtype,
+                       void* workspace, int64_t workspace_bytes, int64_t rows, int64_t cols, void* stream);
 
 /*
  * Log probabilities of given tokens under softmax(logits * inv_temperature), entropies and the best alternatives.

@@ -82,9 +82,16 @@ def lib():
         L.mxq_fp8_quantize.argtypes = [vp, i32, i64, i64, i64, i32, i32, vp, i64, vp, vp, i64, vp, vp, vp]
         L.mxq_sum_partials.argtypes = [vp, i64, i64, vp, i32, vp]
         L.mxq_layer_norm_fwd.argtypes = [vp, i32, i64, vp, vp, i32, vp, vp, vp, i64, i64, f32, vp]
-        L.mxq_layer_norm_partials.argtypes = [i64, i64]
-        L.mxq_layer_norm_partials.restype = i64
-        L.mxq_layer_norm_bwd.argtypes = [vp, vp, i32, i64, i64, vp, i32, vp, vp, vp, vp, i64, i64, vp]
+        L.mxq_layer_norm_workspace_bytes.argtypes = [i64, i64]
+        L.mxq_layer_norm_workspace_bytes.restype = i64
+        L.mxq_layer_norm_bwd.argtypes = [vp, vp, i32, i64, i64, vp, i32, vp, vp, vp, vp, vp, i32, vp, i64, i64, i64, vp]
+        L.mxq_fp8_linear_saved_bytes.argtypes = [i64, i64, i64, i32, i32]
+        L.mxq_fp8_linear_saved_bytes.restype = i64
+        L.mxq_fp8_linear_scratch_bytes.argtypes = [i64, i64, i64, i32]
+        L.mxq_fp8_linear_scratch_bytes.restype = i64
+        L.mxq_fp8_linear_fwd_train.argtypes = [vp, i32, i64, vp, i32, i64, i32, vp, i32, vp, i32, i32, i32, vp, i64, vp, i64, i64, i64,
+                                               i64, vp]
+        L.mxq_fp8_linear_bwd.argtypes = [vp, i32, i64, i32, i32, vp, i64, i32, i32, vp, i32, vp, i32, vp, i32, vp, i64, i64, i64, i64, vp]
         L.mxq_token_logprobs.argtypes = [vp, i32, i64, vp, i64, f32, vp, vp, vp, i32, vp, vp, i64, i64, vp]
         L.mxq_token_logprobs_grad.argtypes = [vp, i32, i64, vp, i64, f32, vp, vp, vp, vp, vp, i64, i64, vp]
         L.mxq_fp8_gemm.argtypes = [vp, i64, vp, i32, i32, vp, i64, vp, i32, i32, vp, i32, vp, i32, i64, i64, i64, vp]
@@ -568,8 +575,10 @@ _F8 = (torch.float8_e4m3fn, torch.float8_e5m2)               # index = the libra
 
 def rows_of(t):
     """t as [rows, last dimension] with unit stride inside a row (a view where the strides allow it)."""
-    t = t.reshape(-1, t.shape[-1]) if t.dim() != 2 else t
-    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    s = t.stride()
+    return t if s[1] == 1 and s[0] >= t.shape[1] else t.contiguous()
 
 
 def fp8_quantize(x, fmt, tile=False, rows=True, cols=False, colsum=False):
@@ -577,19 +586,21 @@ def fp8_quantize(x, fmt, tile=False, rows=True, cols=False, colsum=False):
     operand, column sums [row blocks, columns]; None for what is not asked for.  x: unit stride inside a row."""
     R, C = x.shape
     rb, cb = (R + 127) // 128, (C + 127) // 128
-    u8 = dict(dtype=torch.uint8, device=x.device)
-    f32 = dict(dtype=torch.float32, device=x.device)
     pitch, pitch_t = (C + 15) // 16 * 16, (R + 15) // 16 * 16
-    codes = torch.empty((R, pitch), **u8) if rows else None
-    scales = torch.empty((cb, rb if tile else R), **f32) if rows else None
-    codes_t = torch.empty((C, pitch_t), **u8) if cols else None
-    scales_t = torch.empty((rb, cb if tile else C), **f32) if cols else None
-    sums = torch.empty((rb, C), **f32) if colsum else None
+    codes = codes_t = scales = scales_t = sums = None
+    if rows:
+        codes = x.new_empty((R, pitch), dtype=_F8[fmt])
+        scales = x.new_empty((cb, rb if tile else R), dtype=torch.float32)
+    if cols:
+        codes_t = x.new_empty((C, pitch_t), dtype=_F8[fmt])
+        scales_t = x.new_empty((rb, cb if tile else C), dtype=torch.float32)
+    if colsum:
+        sums = x.new_empty((rb, C), dtype=torch.float32)
     with _device_of(x.device):
-        check(lib().mxq_fp8_quantize(_ptr(x), _DT[x.dtype], R, C, x.stride(0) if R > 1 else C, fmt, int(tile), _ptr(codes), pitch,
+        check(lib().mxq_fp8_quantize(_ptr(x), _DT[x.dtype], R, C, x.stride(0) if R > 1 else C, fmt, tile, _ptr(codes), pitch,
                                      _ptr(scales), _ptr(codes_t), pitch_t, _ptr(scales_t), _ptr(sums), _stream(x)))
-    a = (codes.view(_F8[fmt])[:, :C], scales) if rows else None
-    b = (codes_t.view(_F8[fmt])[:, :R], scales_t) if cols else None
+    a = (codes if pitch == C else codes[:, :C], scales) if rows else None
+    b = (codes_t if pitch_t == R else codes_t[:, :R], scales_t) if cols else None
     return a, b, sums
 
 
@@ -609,55 +620,93 @@ def _pitch(codes):
 def fp8_gemm(a, b, bias, out_dtype):
     """a b^T (+ bias) of two 8-bit block operands (fp8_block.BlockFP8); see mxq_fp8_gemm."""
     (M, K), N = a.codes.shape, b.codes.shape[0]
-    out = torch.empty((M, N), dtype=out_dtype, device=a.codes.device)
+    out = a.codes.new_empty((M, N), dtype=out_dtype)
     with _device_of(out.device):
-        check(lib().mxq_fp8_gemm(_ptr(a.codes), _pitch(a.codes), _ptr(a.scales), int(a.tile), a.fmt, _ptr(b.codes),
-                                 _pitch(b.codes), _ptr(b.scales), int(b.tile), b.fmt, _ptr(out), _DT[out_dtype], _ptr(bias),
+        check(lib().mxq_fp8_gemm(_ptr(a.codes), _pitch(a.codes), _ptr(a.scales), a.tile, a.fmt, _ptr(b.codes),
+                                 _pitch(b.codes), _ptr(b.scales), b.tile, b.fmt, _ptr(out), _DT[out_dtype], _ptr(bias),
                                  _DT[bias.dtype] if bias is not None else 0, M, N, K, _stream(out)))
     return out
 
 
 def fp8_linear_fwd(x, x_fmt, w, bias):
-    """x w^T (+ bias), x [M, K] quantized in the call, w a fp8_block.BlockFP8; see mxq_fp8_linear_fwd."""
+    """x w^T (+ bias), x [M, K] quantized in the call, w an fp8_block.BlockFP8; see mxq_fp8_linear_fwd."""
     (M, K), N = x.shape, w.codes.shape[0]
     L = lib()
-    ws = torch.empty(L.mxq_fp8_linear_workspace_bytes(M, K), dtype=torch.uint8, device=x.device)
-    y = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    size = L.mxq_fp8_linear_workspace_bytes(M, K)
+    ws = x.new_empty(size, dtype=torch.uint8)
+    y = x.new_empty((M, N))
+    dt = _DT[x.dtype]
     with _device_of(x.device):
-        check(L.mxq_fp8_linear_fwd(_ptr(x), _DT[x.dtype], x.stride(0) if M > 1 else K, x_fmt, _ptr(w.codes), _pitch(w.codes),
-                                   _ptr(w.scales), int(w.tile), w.fmt, _ptr(y), _DT[y.dtype], _ptr(bias),
-                                   _DT[bias.dtype] if bias is not None else 0, M, N, K, _ptr(ws), ws.numel(), _stream(x)))
+        check(L.mxq_fp8_linear_fwd(_ptr(x), dt, x.stride(0) if M > 1 else K, x_fmt, _ptr(w.codes), _pitch(w.codes),
+                                   w.scales.data_ptr(), w.tile, w.fmt, _ptr(y), dt, _ptr(bias),
+                                   _DT[bias.dtype] if bias is not None else 0, M, N, K, _ptr(ws), size, _stream(x)))
     return y
+
+
+def fp8_linear_fwd_train(x, w, bias, fmt, need_dx, need_dw):
+    """(y, saved) of x [M, K] and w [N, K], both quantized in the call, M > 0; see mxq_fp8_linear_fwd_train."""
+    (M, K), N = x.shape, w.shape[0]
+    L = lib()
+    keep, size = L.mxq_fp8_linear_saved_bytes(M, N, K, need_dx, need_dw), L.mxq_fp8_linear_scratch_bytes(M, N, K, 0)
+    saved = x.new_empty(keep, dtype=torch.uint8)
+    scratch = x.new_empty(size, dtype=torch.uint8)
+    y = x.new_empty((M, N))
+    dt = _DT[x.dtype]
+    with _device_of(x.device):
+        check(L.mxq_fp8_linear_fwd_train(_ptr(x), dt, x.stride(0) if M > 1 else K, _ptr(w), _DT[w.dtype],
+                                         w.stride(0) if N > 1 else K, fmt, _ptr(bias), _DT[bias.dtype] if bias is not None else 0,
+                                         _ptr(y), dt, need_dx, need_dw, _ptr(saved), keep, _ptr(scratch), size, M, N, K,
+                                         _stream(x)))
+    return y, saved
+
+
+def fp8_linear_bwd(dy, saved, saved_for, grad_fmt, fmt, w_shape, dtypes, need):
+    """(dx, dw, db) of mxq_fp8_linear_fwd_train's layer, None for those not needed; dtypes: of x, w and bias; see mxq_fp8_linear_bwd."""
+    M, (N, K) = dy.shape[0], w_shape
+    L = lib()
+    size = L.mxq_fp8_linear_scratch_bytes(M, N, K, 1)
+    scratch = dy.new_empty(size, dtype=torch.uint8)
+    dx = dy.new_empty((M, K), dtype=dtypes[0]) if need[0] else None
+    dw = dy.new_empty((N, K), dtype=dtypes[1]) if need[1] else None
+    db = dy.new_empty(N, dtype=dtypes[2]) if need[2] else None
+    with _device_of(dy.device):
+        check(L.mxq_fp8_linear_bwd(_ptr(dy), _DT[dy.dtype], dy.stride(0) if M > 1 else N, grad_fmt, fmt, _ptr(saved), saved.numel(),
+                                   saved_for[0], saved_for[1], _ptr(dx), _DT[dtypes[0]], _ptr(dw), _DT[dtypes[1]], _ptr(db),
+                                   _DT[dtypes[2]] if need[2] else 0, _ptr(scratch), size, M, N, K, _stream(dy)))
+    return dx, dw, db
 
 
 def layer_norm_fwd(x, weight, bias, eps, want_saved):
     """(y, mean, rstd) of x [rows, cols] (unit stride inside a row); mean and rstd are None unless wanted; see mxq_layer_norm_fwd."""
     rows, cols = x.shape
-    y = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
+    y = x.new_empty((rows, cols))
     mean = rstd = None
     if want_saved:
-        mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+        mean, rstd = x.new_empty(rows, dtype=torch.float32), x.new_empty(rows, dtype=torch.float32)
     w = weight if weight is not None else bias
+    dt = _DT[x.dtype]
     with _device_of(x.device):
-        check(lib().mxq_layer_norm_fwd(_ptr(x), _DT[x.dtype], x.stride(0) if rows > 1 else cols, _ptr(weight), _ptr(bias),
-                                       _DT[x.dtype if w is None else w.dtype], _ptr(y), _ptr(mean), _ptr(rstd), rows, cols, eps,
+        check(lib().mxq_layer_norm_fwd(_ptr(x), dt, x.stride(0) if rows > 1 else cols, _ptr(weight), _ptr(bias),
+                                       dt if w is None else _DT[w.dtype], _ptr(y), _ptr(mean), _ptr(rstd), rows, cols, eps,
                                        _stream(x)))
     return y, mean, rstd
 
 
-def layer_norm_bwd(dy, x, weight, mean, rstd, want_dx, want_sums):
-    """(dx or None, partial sums of dw and db [CTAs, 2 * cols] or None); see mxq_layer_norm_bwd."""
+def layer_norm_bwd(dy, x, weight, mean, rstd, sums_dtype, need):
+    """(dx, dw, db) of layer_norm_fwd, None for those not needed; see mxq_layer_norm_bwd."""
     rows, cols = x.shape
-    dx = torch.empty((rows, cols), dtype=x.dtype, device=x.device) if want_dx else None
     L = lib()
+    dx = x.new_empty((rows, cols)) if need[0] else None
+    dw = x.new_empty(cols, dtype=sums_dtype) if need[1] else None
+    db = x.new_empty(cols, dtype=sums_dtype) if need[2] else None
+    dt = _DT[x.dtype]
     with _device_of(x.device):
-        part = torch.empty((L.mxq_layer_norm_partials(rows, cols), 2 * cols), dtype=torch.float32, device=x.device) \
-            if want_sums else None
-        check(L.mxq_layer_norm_bwd(_ptr(dy), _ptr(x), _DT[x.dtype], dy.stride(0) if rows > 1 else cols,
-                                   x.stride(0) if rows > 1 else cols, _ptr(weight),
-                                   _DT[x.dtype if weight is None else weight.dtype], _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(part),
-                                   rows, cols, _stream(x)))
-    return dx, part
+        size = L.mxq_layer_norm_workspace_bytes(rows, cols) if need[1] or need[2] else 0
+        ws = x.new_empty(size, dtype=torch.uint8) if size else None
+        check(L.mxq_layer_norm_bwd(_ptr(dy), _ptr(x), dt, dy.stride(0) if rows > 1 else cols, x.stride(0) if rows > 1 else cols,
+                                   _ptr(weight), dt if weight is None else _DT[weight.dtype], _ptr(mean), _ptr(rstd), _ptr(dx),
+                                   _ptr(dw), _ptr(db), _DT[sums_dtype], _ptr(ws), size, rows, cols, _stream(x)))
+    return dx, dw, db
 
 
 LOGPROBS_MAX_TOP = 32
@@ -666,12 +715,11 @@ LOGPROBS_MAX_TOP = 32
 def token_logprobs(x, tokens, ignore_index, inv_t, entropy, top, want_lse):
     """(logprobs, entropy, lse, top logprobs, top tokens) of x [rows, vocab]; None for what is not wanted; see mxq_token_logprobs."""
     rows, vocab = x.shape
-    f32 = dict(dtype=torch.float32, device=x.device)
-    lp = torch.empty(rows, **f32) if tokens is not None else None
-    h = torch.empty(rows, **f32) if entropy else None
-    lse = torch.empty(rows, **f32) if want_lse else None
-    tlp = torch.empty((rows, top), **f32) if top else None
-    tok = torch.empty((rows, top), dtype=torch.int64, device=x.device) if top else None
+    lp = x.new_empty(rows, dtype=torch.float32) if tokens is not None else None
+    h = x.new_empty(rows, dtype=torch.float32) if entropy else None
+    lse = x.new_empty(rows, dtype=torch.float32) if want_lse else None
+    tlp = x.new_empty((rows, top), dtype=torch.float32) if top else None
+    tok = x.new_empty((rows, top), dtype=torch.int64) if top else None
     with _device_of(x.device):
         check(lib().mxq_token_logprobs(_ptr(x), _DT[x.dtype], x.stride(0) if rows > 1 else vocab, _ptr(tokens), ignore_index, inv_t,
                                        _ptr(lp), _ptr(h), _ptr(lse), top, _ptr(tlp), _ptr(tok), rows, vocab, _stream(x)))
@@ -681,7 +729,7 @@ def token_logprobs(x, tokens, ignore_index, inv_t, entropy, top, want_lse):
 def token_logprobs_grad(x, tokens, ignore_index, inv_t, lse, entropy, g_lp, g_h):
     """Gradient [rows, vocab] with respect to x; see mxq_token_logprobs_grad."""
     rows, vocab = x.shape
-    dx = torch.empty((rows, vocab), dtype=x.dtype, device=x.device)
+    dx = x.new_empty((rows, vocab))
     with _device_of(x.device):
         check(lib().mxq_token_logprobs_grad(_ptr(x), _DT[x.dtype], x.stride(0) if rows > 1 else vocab, _ptr(tokens), ignore_index,
                                             inv_t, _ptr(lse), _ptr(entropy), _ptr(g_lp), _ptr(g_h), _ptr(dx), rows, vocab,

@@ -310,3 +310,108 @@ extern "C" int mxq_fp8_linear_fwd(const void* x, int x_dtype, int64_t x_stride, 
     return mxq_fp8_gemm(workspace, pitch, scales, 0, x_fmt, w, w_pitch, w_scales, w_tile, w_fmt, y, y_dtype, bias, bias_dtype,
                         M, N, K, stream);
 }
+
+// ---------------------------------------------------------------------------------------------------------------
+// A linear layer's training step as one call each way.  `saved` holds what the backward pass needs of the forward one's
+// operands (x transposed for dw, w transposed for dx), `scratch` what only the running call needs.
+// ---------------------------------------------------------------------------------------------------------------
+namespace mxq {
+struct Carve {                                     // hands out 256-byte aligned parts of one buffer
+    uint8_t* base;
+    int64_t used = 0;
+    explicit Carve(void* p) : base(static_cast<uint8_t*>(p)) {}
+    uint8_t* take(int64_t bytes) {
+        uint8_t* p = base ? base + used : nullptr;
+        used += (bytes + 255) / 256 * 256;
+        return p;
+    }
+};
+struct Operand8 { uint8_t* codes = nullptr; int64_t pitch = 0; float* scales = nullptr; };
+static Operand8 carve_operand(Carve& c, int64_t rows, int64_t K, bool tile) {
+    Operand8 o;
+    o.pitch = (K + 15) / 16 * 16;
+    o.codes = c.take(rows * o.pitch);
+    o.scales = reinterpret_cast<float*>(c.take(4 * ((K + 127) / 128) * (tile ? (rows + 127) / 128 : rows)));
+    return o;
+}
+struct Saved8 { Operand8 xt, wt; int64_t bytes; };
+static Saved8 carve_saved(void* p, int64_t M, int64_t N, int64_t K, int need_dx, int need_dw) {
+    Carve c(p);
+    Saved8 s;
+    if (need_dw) s.xt = carve_operand(c, K, M, false);
+    if (need_dx) s.wt = carve_operand(c, K, N, true);
+    s.bytes = c.used;
+    return s;
+}
+struct Scratch8 { Operand8 x, w; int64_t bytes; };
+static Scratch8 carve_fwd(void* p, int64_t M, int64_t N, int64_t K) {
+    Carve c(p);
+    Scratch8 s;
+    s.x = carve_operand(c, M, K, false);
+    s.w = carve_operand(c, N, K, true);
+    s.bytes = c.used;
+    return s;
+}
+struct Grads8 { Operand8 dy, dyt; float* sums; int64_t bytes; };
+static Grads8 carve_bwd(void* p, int64_t M, int64_t N, int64_t K) {
+    Carve c(p);
+    Grads8 s;
+    s.dy = carve_operand(c, M, N, false);
+    s.dyt = carve_operand(c, N, M, false);
+    s.sums = reinterpret_cast<float*>(c.take(4 * ((M + 127) / 128) * N));
+    s.bytes = c.used;
+    return s;
+}
+}  // namespace mxq
+
+extern "C" int64_t mxq_fp8_linear_saved_bytes(int64_t M, int64_t N, int64_t K, int need_dx, int need_dw) {
+    return M < 0 || N < 0 || K < 0 ? -1 : mxq::carve_saved(nullptr, M, N, K, need_dx, need_dw).bytes;
+}
+extern "C" int64_t mxq_fp8_linear_scratch_bytes(int64_t M, int64_t N, int64_t K, int backward) {
+    if (M < 0 || N < 0 || K < 0) return -1;
+    return backward ? mxq::carve_bwd(nullptr, M, N, K).bytes : mxq::carve_fwd(nullptr, M, N, K).bytes;
+}
+
+extern "C" int mxq_fp8_linear_fwd_train(const void* x, int x_dtype, int64_t x_stride, const void* w, int w_dtype, int64_t w_stride,
+                                        int fmt, const void* bias, int bias_dtype, void* y, int y_dtype, int need_dx, int need_dw,
+                                        void* saved, int64_t saved_bytes, void* scratch, int64_t scratch_bytes, int64_t M, int64_t N,
+                                        int64_t K, void* stream) {
+    using namespace mxq;
+    if (M <= 0 || N <= 0 || K <= 0 || !scratch || ((need_dx || need_dw) && !saved)) return MXQ_ERR_BAD_ARG;
+    if ((reinterpret_cast<uintptr_t>(scratch) | reinterpret_cast<uintptr_t>(saved)) & 255) return MXQ_ERR_ALIGN;
+    const Scratch8 q = carve_fwd(scratch, M, N, K);
+    const Saved8 s = carve_saved(saved, M, N, K, need_dx, need_dw);
+    if (scratch_bytes < q.bytes || saved_bytes < s.bytes) return MXQ_ERR_BAD_ARG;
+    int rc = mxq_fp8_quantize(x, x_dtype, M, K, x_stride, fmt, 0, q.x.codes, q.x.pitch, q.x.scales, s.xt.codes, s.xt.pitch, s.xt.scales,
+                              nullptr, stream);
+    if (rc) return rc;
+    rc = mxq_fp8_quantize(w, w_dtype, N, K, w_stride, fmt, 1, q.w.codes, q.w.pitch, q.w.scales, s.wt.codes, s.wt.pitch, s.wt.scales,
+                          nullptr, stream);
+    if (rc) return rc;
+    return mxq_fp8_gemm(q.x.codes, q.x.pitch, q.x.scales, 0, fmt, q.w.codes, q.w.pitch, q.w.scales, 1, fmt, y, y_dtype, bias, bias_dtype,
+                        M, N, K, stream);
+}
+
+extern "C" int mxq_fp8_linear_bwd(const void* dy, int dy_dtype, int64_t dy_stride, int grad_fmt, int fmt, const void* saved,
+                                  int64_t saved_bytes, int saved_dx, int saved_dw, void* dx, int dx_dtype, void* dw, int dw_dtype,
+                                  void* db, int db_dtype, void* scratch, int64_t scratch_bytes, int64_t M, int64_t N, int64_t K,
+                                  void* stream) {
+    using namespace mxq;
+    if (M <= 0 || N <= 0 || K <= 0 || (dx && !saved_dx) || (dw && !saved_dw)) return MXQ_ERR_BAD_ARG;
+    if (!dx && !dw && !db) return MXQ_OK;
+    if (!scratch || ((dx || dw) && !saved)) return MXQ_ERR_BAD_ARG;
+    if ((reinterpret_cast<uintptr_t>(scratch) | reinterpret_cast<uintptr_t>(saved)) & 255) return MXQ_ERR_ALIGN;
+    const Grads8 q = carve_bwd(scratch, M, N, K);
+    const Saved8 s = carve_saved(const_cast<void*>(saved), M, N, K, saved_dx, saved_dw);
+    if (scratch_bytes < q.bytes || ((dx || dw) && saved_bytes < s.bytes)) return MXQ_ERR_BAD_ARG;
+    int rc = mxq_fp8_quantize(dy, dy_dtype, M, N, dy_stride, grad_fmt, 0, dx || !dw ? q.dy.codes : nullptr, q.dy.pitch, q.dy.scales,
+                              dw ? q.dyt.codes : nullptr, q.dyt.pitch, q.dyt.scales, db ? q.sums : nullptr, stream);
+    if (!rc && dx)
+        rc = mxq_fp8_gemm(q.dy.codes, q.dy.pitch, q.dy.scales, 0, grad_fmt, s.wt.codes, s.wt.pitch, s.wt.scales, 1, fmt, dx, dx_dtype,
+                          nullptr, 0, M, K, N, stream);
+    if (!rc && dw)
+        rc = mxq_fp8_gemm(q.dyt.codes, q.dyt.pitch, q.dyt.scales, 0, grad_fmt, s.xt.codes, s.xt.pitch, s.xt.scales, 0, fmt, dw, dw_dtype,
+                          nullptr, 0, N, K, M, stream);
+    if (!rc && db) rc = mxq_sum_partials(q.sums, (M + 127) / 128, N, db, db_dtype, stream);
+    return rc;
+}

@@ -200,31 +200,45 @@ fp8_quantize_kernel(const QuantArgs g, const bool tile) {
     }
 }
 
-// out[c] = sum over n partial rows of part[., c], added in order; one thread per column.
+// Column sums of part [n, pitch]: 32 columns a CTA, each of its 8 warps adds every eighth row (four at a time in flight),
+// and the warps' sums are added in order.
 template <int DT>
-__global__ void __launch_bounds__(256) sum_partials_kernel(const float* part, int64_t n, int64_t cols, void* out) {
-    const int64_t c = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
+__global__ void __launch_bounds__(256)
+sum_partials_kernel(const float* part, int64_t n, int64_t cols, int64_t pitch, void* out0, void* out1) {
+    const int set = blockIdx.y;
+    void* out = set ? out1 : out0;
+    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t c = (int64_t)blockIdx.x * 32 + lane;
     __shared__ float s[8][32];
-    const int w = threadIdx.x >> 5;
-    float a = 0.f;
-    if (c < cols)
-        for (int64_t i = w; i < n; i += 8) a += part[i * cols + c];
-    s[w][threadIdx.x & 31] = a;
+    if (!out) return;
+    const float* p = part + set * cols + c;
+    float a[4] = {0.f, 0.f, 0.f, 0.f};
+    if (c < cols) {
+        int64_t i = w;
+        for (; i + 24 < n; i += 32) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) a[j] += p[(i + 8 * j) * pitch];
+        }
+        for (; i < n; i += 8) a[0] += p[i * pitch];
+    }
+    s[w][lane] = (a[0] + a[1]) + (a[2] + a[3]);
     __syncthreads();
     if (w == 0 && c < cols) {
+        float v = s[0][lane];
 #pragma unroll
-        for (int i = 1; i < 8; ++i) a += s[i][threadIdx.x & 31];
-        store1<DT>(out, c, a);
+        for (int i = 1; i < 8; ++i) v += s[i][lane];
+        store1<DT>(out, c, v);
     }
 }
 
-int sum_partials(const float* part, int64_t n, int64_t cols, void* out, int dtype, cudaStream_t st) {
+int sum_partials(const float* part, int64_t n, int64_t cols, int sets, void* out0, void* out1, int dtype, cudaStream_t st) {
     if (cols <= 0) return MXQ_OK;
     const int64_t grid = (cols + 31) / 32;
     if (grid > 0x7fffffff) return MXQ_ERR_TOO_LARGE;
-    if (dtype == MXQ_F32) sum_partials_kernel<DT_F32><<<(int)grid, 256, 0, st>>>(part, n, cols, out);
-    else if (dtype == MXQ_F16) sum_partials_kernel<DT_F16><<<(int)grid, 256, 0, st>>>(part, n, cols, out);
-    else if (dtype == MXQ_BF16) sum_partials_kernel<DT_BF16><<<(int)grid, 256, 0, st>>>(part, n, cols, out);
+    const dim3 g((unsigned)grid, (unsigned)sets);
+    if (dtype == MXQ_F32) sum_partials_kernel<DT_F32><<<g, 256, 0, st>>>(part, n, cols, sets * cols, out0, out1);
+    else if (dtype == MXQ_F16) sum_partials_kernel<DT_F16><<<g, 256, 0, st>>>(part, n, cols, sets * cols, out0, out1);
+    else if (dtype == MXQ_BF16) sum_partials_kernel<DT_BF16><<<g, 256, 0, st>>>(part, n, cols, sets * cols, out0, out1);
     else return MXQ_ERR_BAD_ARG;
     return check_launch();
 }
@@ -262,5 +276,5 @@ extern "C" int mxq_fp8_quantize(const void* x, int dtype, int64_t rows, int64_t 
 
 extern "C" int mxq_sum_partials(const float* part, int64_t n, int64_t cols, void* out, int dtype, void* stream) {
     if (n < 0 || cols < 0 || (cols > 0 && (!out || (n > 0 && !part)))) return MXQ_ERR_BAD_ARG;
-    return mxq::sum_partials(part, n, cols, out, dtype, (cudaStream_t)stream);
+    return mxq::sum_partials(part, n, cols, 1, out, nullptr, dtype, (cudaStream_t)stream);
 }

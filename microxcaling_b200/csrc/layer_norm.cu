@@ -393,19 +393,26 @@ extern "C" int mxq_layer_norm_fwd(const void* x, int dtype, int64_t x_stride, co
     return norm_dispatch(g, dtype, w_dtype, false, (cudaStream_t)stream);
 }
 
-extern "C" int64_t mxq_layer_norm_partials(int64_t rows, int64_t cols) {
-    return rows <= 0 || cols <= 0 ? 0 : mxq::norm_bwd_ctas(rows, cols);
+extern "C" int64_t mxq_layer_norm_workspace_bytes(int64_t rows, int64_t cols) {
+    return rows <= 0 || cols <= 0 ? 0 : mxq::norm_bwd_ctas(rows, cols) * 8 * cols;
 }
 
 extern "C" int mxq_layer_norm_bwd(const void* dy, const void* x, int dtype, int64_t dy_stride, int64_t x_stride, const void* w, int w_dtype,
-                                  const float* mean, const float* rstd, void* dx, float* partials, int64_t rows, int64_t cols,
-                                  void* stream) {
+                                  const float* mean, const float* rstd, void* dx, void* dw, void* db, int sums_dtype, void* workspace,
+                                  int64_t workspace_bytes, int64_t rows, int64_t cols, void* stream) {
     using namespace mxq;
-    if (rows < 0 || cols <= 0 || dtype < 0 || dtype > 2 || w_dtype < 0 || w_dtype > 2) return MXQ_ERR_BAD_ARG;
-    if (rows == 0 || (!dx && !partials)) return MXQ_OK;
+    if (rows < 0 || cols <= 0 || dtype < 0 || dtype > 2 || w_dtype < 0 || w_dtype > 2 || sums_dtype < 0 || sums_dtype > 2) return MXQ_ERR_BAD_ARG;
+    if (!dx && !dw && !db) return MXQ_OK;
+    cudaStream_t st = (cudaStream_t)stream;
+    const bool sums = dw || db;
+    if (rows == 0) return sum_partials(nullptr, 0, cols, 2, dw, db, sums_dtype, st);
     if (!x || !dy || !mean || !rstd || (rows > 1 && (x_stride < cols || dy_stride < cols))) return MXQ_ERR_BAD_ARG;
+    if (sums && (!workspace || workspace_bytes < mxq_layer_norm_workspace_bytes(rows, cols))) return MXQ_ERR_BAD_ARG;
+    if (sums && !aligned16(workspace)) return MXQ_ERR_ALIGN;
     NormArgs g = {};
-    g.x = x; g.dy = dy; g.w = w; g.out = dx; g.mean = const_cast<float*>(mean); g.rstd = const_cast<float*>(rstd); g.part = partials;
+    g.x = x; g.dy = dy; g.w = w; g.out = dx; g.mean = const_cast<float*>(mean); g.rstd = const_cast<float*>(rstd);
+    g.part = sums ? (float*)workspace : nullptr;
     g.rows = rows; g.cols = cols; g.x_stride = x_stride; g.dy_stride = dy_stride;
-    return norm_dispatch(g, dtype, w_dtype, true, (cudaStream_t)stream);
+    const int rc = norm_dispatch(g, dtype, w_dtype, true, st);
+    return rc || !sums ? rc : sum_partials(g.part, norm_bwd_ctas(rows, cols), cols, 2, dw, db, sums_dtype, st);
 }

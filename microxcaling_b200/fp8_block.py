@@ -16,7 +16,7 @@ of this in the reference."""
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._autograd import call
+from . import _backend
 from ._backend import MxqError
 
 FORMATS = ("fp8_e4m3", "fp8_e5m2")                       # index = the library's format id
@@ -106,7 +106,6 @@ def _host_quantize(x, fmt, tile):
 def _quantize(x, fmt, tile, rows, cols, colsum=False):
     """x [rows, K] -> (operand or None, transposed operand or None, column sums [n, K] in fp32 or None)"""
     if x.is_cuda:
-        from . import _backend
         x = _backend.rows_of(x)
         if x.shape[0] == 0:                              # nothing to launch: sums over no rows are zero
             sums = torch.zeros((1, x.shape[1]), dtype=torch.float32, device=x.device) if colsum else None
@@ -133,11 +132,14 @@ def quantize_fp8_block(x, elem_format="fp8_e4m3", axes=-1, tile=False):
     fmt = _fmt(elem_format)
     _check_float(x, "x")
     want = (axes,) if isinstance(axes, int) else tuple(axes)
-    if not want or any(a not in (-1, -2) for a in want) or len(set(want)) != len(want):
+    if want not in ((-1,), (-2,), (-1, -2), (-2, -1)):
         raise MxqError("axes must be -1, -2 or both, not %r" % (axes,))
     if x.dim() == 0 or x.shape[-1] == 0:
         raise MxqError("x needs at least one value along its last dimension")
-    x = x.detach().reshape(-1, x.shape[-1])
+    if x.requires_grad:
+        x = x.detach()
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
     if -2 in want and x.shape[0] == 0:
         raise MxqError("blocks along the rows need at least one row")
     a, b, _ = _quantize(x, fmt, bool(tile), -1 in want, -2 in want)
@@ -146,13 +148,12 @@ def quantize_fp8_block(x, elem_format="fp8_e4m3", axes=-1, tile=False):
 
 
 def _check_bias(bias, n, device):
-    if bias is not None and (bias.dtype not in _FLOATS or bias.shape != (n,) or bias.device != device or not bias.is_contiguous()):
+    if bias is not None and (bias.dtype not in _FLOATS or bias.shape != (n,) or bias.device != device or bias.stride(0) != 1 and n > 1):
         raise MxqError("bias must be a contiguous float tensor of %d values on the operands' device" % n)
 
 
 def _matmul(a, b, bias, out_dtype):
     if a.codes.is_cuda:
-        from . import _backend
         return _backend.fp8_gemm(a, b, bias, out_dtype)
     y = a.dequantize() @ b.dequantize().t()
     return (y if bias is None else y + bias.float()).to(out_dtype)
@@ -173,57 +174,84 @@ def fp8_block_matmul(a, b, bias=None, out_dtype=torch.bfloat16):
     return _matmul(a, b, bias.detach() if bias is not None else None, out_dtype)
 
 
-class Fp8BlockLinearFunction(torch.autograd.Function):
+def _forward(x2, w, bias, fmt):
+    """x2 [tokens, K] times a packed weight, no gradient."""
+    if x2.is_cuda:
+        return _backend.fp8_linear_fwd(_backend.rows_of(x2), fmt, w, bias)
+    return _matmul(_quantize(x2, fmt, False, True, False)[0], w, bias, x2.dtype)
+
+
+class PackedLinearFunction(torch.autograd.Function):
+    """The layer with a weight that was packed before: gradients of x and bias."""
+
     @staticmethod
-    def forward(ctx, x, weight, bias, fmt, grad_fmt):
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        packed = isinstance(weight, BlockFP8)
-        x2 = x.reshape(-1, x.shape[-1])
-        wt = None
-        if packed:
-            w, wt = weight, weight.transposed
-            if need_x and wt is None:
+    def forward(ctx, x, bias, w, fmt, grad_fmt):
+        wt = w.transposed
+        if ctx.needs_input_grad[0]:
+            if wt is None:
                 raise MxqError("the gradient of x needs a packed weight that carries its transposed operand")
-        else:
-            w, wt, _ = _quantize(weight, fmt, True, True, need_x)
-        xt = None
-        if x.is_cuda and not need_w:
-            from . import _backend
-            y = _backend.fp8_linear_fwd(_backend.rows_of(x2), fmt, w, bias)
-        else:
-            q, xt, _ = _quantize(x2, fmt, False, True, need_w and x2.shape[0] > 0)
-            y = _matmul(q, w, bias, x.dtype)
-        keep = (xt, wt if need_x else None)
-        ctx.save_for_backward(*[t for o in keep for t in ((None, None) if o is None else (o.codes, o.scales))])
-        ctx.fmts = (fmt, None if wt is None else wt.fmt)
-        ctx.grad_fmt, ctx.x_shape = grad_fmt, x.shape
-        ctx.dtypes = (x.dtype, None if packed else weight.dtype, None if bias is None else bias.dtype)
-        ctx.w_shape = tuple(w.codes.shape)
-        return y.reshape(*x.shape[:-1], w.codes.shape[0])
+            ctx.save_for_backward(wt.codes, wt.scales)
+            ctx.wt_kind = (wt.tile, wt.fmt)
+        ctx.args = (grad_fmt, x.shape, x.dtype, None if bias is None else bias.dtype)
+        return _forward(x.reshape(-1, x.shape[-1]), w, bias, fmt).view(*x.shape[:-1], w.codes.shape[0])
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        xc, xs, wc, ws = ctx.saved_tensors
-        xt = None if xc is None else _operand((xc, xs), False, ctx.fmts[0])
-        wt = None if wc is None else _operand((wc, ws), True, ctx.fmts[1])
-        dy2 = dy.reshape(-1, dy.shape[-1])
-        dx = dw = db = None
-        q, qt, sums = _quantize(dy2, ctx.grad_fmt, False, need_x or not need_w, need_w and xt is not None, need_b)
+        need_x, need_b = ctx.needs_input_grad[:2]
+        grad_fmt, x_shape, x_dtype, b_dtype = ctx.args
+        q, _, sums = _quantize(dy.reshape(-1, dy.shape[-1]), grad_fmt, False, True, False, need_b)
+        dx = db = None
         if need_x:
-            dx = _matmul(q, wt, None, ctx.dtypes[0]).reshape(ctx.x_shape)
-        if need_w:
-            if xt is not None:
-                dw = _matmul(qt, xt, None, ctx.dtypes[1])
-            else:                                            # no tokens
-                dw = torch.zeros(ctx.w_shape, dtype=ctx.dtypes[1], device=dy.device)
+            wt = BlockFP8.__new__(BlockFP8)._set(*ctx.saved_tensors, *ctx.wt_kind)
+            dx = _matmul(q, wt, None, x_dtype).view(x_shape)
         if need_b:
-            if dy.is_cuda:
-                from . import _backend
-                db = _backend.sum_partials(sums, ctx.dtypes[2])
-            else:
-                db = sums[0].to(ctx.dtypes[2])
+            db = _backend.sum_partials(sums, b_dtype) if dy.is_cuda else sums[0].to(b_dtype)
+        return dx, db, None, None, None
+
+
+class Fp8BlockLinearFunction(torch.autograd.Function):
+    """The layer with its weight quantized in the call, which keeps the transposed operands for the gradients."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, fmt, grad_fmt):
+        x2 = x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x
+        n = weight.shape[0]
+        ctx.args = (fmt, grad_fmt, ctx.needs_input_grad[:2], x.shape, tuple(weight.shape),
+                    (x.dtype, weight.dtype, None if bias is None else bias.dtype))
+        if x.is_cuda and x2.shape[0] > 0:
+            y, saved = _backend.fp8_linear_fwd_train(_backend.rows_of(x2), _backend.rows_of(weight), bias, fmt,
+                                                     *ctx.needs_input_grad[:2])
+            ctx.save_for_backward(saved)
+        else:
+            ctx.save_for_backward(x2, weight)
+            w, _, _ = _quantize(weight, fmt, True, True, False)
+            y = _matmul(_quantize(x2, fmt, False, True, False)[0], w, bias, x.dtype)
+        return y if x.dim() == 2 else y.view(*x.shape[:-1], n)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        fmt, grad_fmt, saved_for, x_shape, w_shape, dtypes = ctx.args
+        need = ctx.needs_input_grad[:3]
+        dy2 = dy.reshape(-1, dy.shape[-1]) if dy.dim() != 2 else dy
+        if len(ctx.saved_tensors) == 1:
+            dx, dw, db = _backend.fp8_linear_bwd(_backend.rows_of(dy2), ctx.saved_tensors[0], saved_for, grad_fmt, fmt, w_shape,
+                                                 dtypes, need)
+            return dx.view(x_shape) if need[0] and len(x_shape) != 2 else dx, dw, db, None, None
+        x2, weight = ctx.saved_tensors
+        if dy2.shape[0] == 0:                                # no tokens
+            dx, dw, db = (dy.new_zeros(s, dtype=t) if n else None
+                          for s, t, n in zip((x_shape, w_shape, w_shape[:1]), dtypes, need))
+            return dx, dw, db, None, None
+        dx = dw = db = None
+        if need[0]:
+            dx = _matmul(_quantize(dy2, grad_fmt, False, True, False)[0], _quantize(weight, fmt, True, False, True)[1], None,
+                         dtypes[0]).view(x_shape)
+        if need[1]:
+            dw = _matmul(_quantize(dy2, grad_fmt, False, False, True)[1], _quantize(x2, fmt, False, False, True)[1], None, dtypes[1])
+        if need[2]:
+            db = dy2.float().sum(0).to(dtypes[2])
         return dx, dw, db, None, None
 
 
@@ -237,18 +265,29 @@ def fp8_block_linear(x, weight, bias=None, elem_format="fp8_e4m3", grad_elem_for
     fmt, grad_fmt = _fmt(elem_format), _fmt(grad_elem_format)
     _check_float(x, "x")
     packed = isinstance(weight, BlockFP8)
-    if not packed:
+    if packed:
+        (n, k), dev = weight.codes.shape, weight.codes.device
+    else:
         _check_float(weight, "weight")
         if weight.dim() != 2:
             raise MxqError("weight must be 2-D")
-    n, k = weight.shape
+        (n, k), dev = weight.shape, weight.device
     if x.dim() == 0 or x.shape[-1] != k or k == 0 or n == 0:
         raise MxqError("x %s does not fit a weight [%d, %d]" % (list(x.shape), n, k))
-    dev = weight.codes.device if packed else weight.device
     if x.device != dev:
         raise MxqError("x and weight are on different devices")
-    _check_bias(bias, n, dev)
-    return call(Fp8BlockLinearFunction, x, weight, bias, fmt, grad_fmt)
+    if bias is not None:
+        _check_bias(bias, n, dev)
+    grad = torch.is_grad_enabled() and (x.requires_grad or not packed and weight.requires_grad or
+                                        bias is not None and bias.requires_grad)
+    if grad:
+        return PackedLinearFunction.apply(x, bias, weight, fmt, grad_fmt) if packed else \
+            Fp8BlockLinearFunction.apply(x, weight, bias, fmt, grad_fmt)
+    with torch.no_grad():
+        w = weight if packed else _quantize(weight, fmt, True, True, False)[0]
+        if x.dim() == 2:
+            return _forward(x, w, bias, fmt)
+        return _forward(x.reshape(-1, k), w, bias, fmt).view(*x.shape[:-1], n)
 
 
 class Fp8BlockLinear(torch.nn.Linear):

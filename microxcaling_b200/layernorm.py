@@ -4,6 +4,7 @@ emulates no vector format, computed in fp32 in one pass each way and rounded onc
 import torch
 from torch.autograd.function import once_differentiable
 
+from . import _backend
 from ._autograd import call
 from ._backend import MxqError
 from .norm_utils import norm_backward_ln, norm_forward
@@ -17,7 +18,6 @@ class RMSNormFunction(torch.autograd.Function):
     def forward(ctx, x, weight, bias, eps, mx_specs=None, name=None):
         sp = mx_specs
         if fused_bf16_ok(sp, x, weight, bias) and x.shape[-1] == weight.numel() == bias.numel():
-            from . import _backend
             if any(ctx.needs_input_grad[:3]):
                 out, x_norm, rms_inv = _backend.rmsnorm_bf16(x.contiguous(), weight.contiguous(), bias.contiguous(),
                                                              eps, want_saved=True)
@@ -129,48 +129,50 @@ def layer_norm(input, normalized_shape, weight, bias, eps=1e-12, mx_specs=None, 
 class FusedLayerNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        from . import _backend
         x2 = _backend.rows_of(x)
-        want = any(ctx.needs_input_grad[:3])
-        y, mean, rstd = _backend.layer_norm_fwd(x2, weight, bias, eps, want)
-        if want:
-            ctx.save_for_backward(x2, weight, mean, rstd)
-            ctx.bias_dtype = None if bias is None else bias.dtype
-        return y.view(x.shape)
+        y, mean, rstd = _backend.layer_norm_fwd(x2, weight, bias, eps, True)
+        ctx.save_for_backward(x2, weight, mean, rstd)
+        ctx.sums_dtype = x.dtype if weight is None and bias is None else (bias if weight is None else weight).dtype
+        return y if x.dim() == 2 else y.view(x.shape)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        from . import _backend
         x2, weight, mean, rstd = ctx.saved_tensors
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dx, part = _backend.layer_norm_bwd(_backend.rows_of(dy), x2, weight, mean, rstd, need_x, need_w or need_b)
-        dw = db = None
-        if part is not None:
-            sums = _backend.sum_partials(part, weight.dtype if weight is not None else ctx.bias_dtype)
-            cols = x2.shape[1]
-            dw, db = sums[:cols] if need_w else None, sums[cols:] if need_b else None
-        return dx.view(dy.shape) if need_x else None, dw, db, None
+        need = ctx.needs_input_grad[:3]
+        dx, dw, db = _backend.layer_norm_bwd(_backend.rows_of(dy), x2, weight, mean, rstd, ctx.sums_dtype, need)
+        return dx.view(dy.shape) if need[0] and dy.dim() != 2 else dx, dw, db, None
+
+
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
 
 def fused_layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension, in fp32 and rounded once to x's dtype; no
     vector format is emulated (layer_norm does that).  weight and bias: [cols], both of x's dtype or both float32; either may be
     None.  Gradients: dx of x's dtype; dw and db summed over the rows in fp32, in a fixed order."""
-    if not isinstance(x, torch.Tensor) or x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+    if not isinstance(x, torch.Tensor) or x.dtype not in _FLOATS:
         raise MxqError("x must be a float32, float16 or bfloat16 tensor")
     if x.dim() == 0 or x.shape[-1] == 0:
         raise MxqError("x needs at least one value along its last dimension")
     if not eps >= 0:
         raise MxqError("eps must not be negative")
+    grad = x.requires_grad
     for t, name in ((weight, "weight"), (bias, "bias")):
-        if t is not None and (t.shape != x.shape[-1:] or t.dtype not in (x.dtype, torch.float32) or t.device != x.device or
-                              not t.is_contiguous()):
-            raise MxqError("%s must be a contiguous tensor of %d values of x's dtype or float32 on x's device" % (name, x.shape[-1]))
+        if t is not None:
+            if t.shape != x.shape[-1:] or t.dtype not in (x.dtype, torch.float32) or t.device != x.device or not t.is_contiguous():
+                raise MxqError("%s must be a contiguous tensor of %d values of x's dtype or float32 on x's device" %
+                               (name, x.shape[-1]))
+            grad = grad or t.requires_grad
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise MxqError("weight and bias must have one dtype")
     if x.is_cuda:
-        return call(FusedLayerNormFunction, x, weight, bias, float(eps))
+        if grad and torch.is_grad_enabled():
+            return FusedLayerNormFunction.apply(x, weight, bias, float(eps))
+        if x.dim() == 2:
+            return _backend.layer_norm_fwd(_backend.rows_of(x), weight, bias, float(eps), False)[0]
+        with torch.no_grad():
+            return _backend.layer_norm_fwd(_backend.rows_of(x), weight, bias, float(eps), False)[0].view(x.shape)
     v = x.float()
     d = v - v.mean(-1, keepdim=True)
     y = d / ((d * d).mean(-1, keepdim=True) + eps).sqrt()

@@ -8,34 +8,38 @@ import collections
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._autograd import call
+from . import _backend
 from ._backend import LOGPROBS_MAX_TOP, MxqError
 
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 TokenLogprobs = collections.namedtuple("TokenLogprobs", "logprobs entropy top_logprobs top_tokens")
+
+
+def _run(x, tokens, top, entropy, inv_t, ignore_index, want_lse):
+    """(rows of x, tokens, log sum, entropy as the kernel wrote them; the outputs in the shape of x's leading dimensions)"""
+    x2 = _backend.rows_of(x)
+    t = None if tokens is None else tokens.reshape(-1).contiguous()
+    lp, h, lse, tlp, tok = _backend.token_logprobs(x2, t, ignore_index, inv_t, entropy, top, want_lse)
+    out = (lp, h, tlp, tok)
+    if x.dim() != 2:
+        out = tuple(None if o is None else o.view(x.shape[:-1] + o.shape[1:]) for o in out)
+    return x2, t, lse, h, out
 
 
 class TokenLogprobsFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, tokens, top, entropy, inv_t, ignore_index):
-        from . import _backend
-        x2 = _backend.rows_of(x)
-        want = ctx.needs_input_grad[0]
-        t = None if tokens is None else tokens.reshape(-1)
-        lp, h, lse, tlp, tok = _backend.token_logprobs(x2, t, ignore_index, inv_t, entropy, top, want)
-        if want:
-            ctx.save_for_backward(x2, t, lse, h)
-            ctx.args = (inv_t, ignore_index, x.shape)
-            ctx.set_materialize_grads(False)
-        lead = x.shape[:-1]
-        lp, h, tlp, tok = (None if o is None else o.view(lead + o.shape[1:]) for o in (lp, h, tlp, tok))
+        x2, t, lse, h, out = _run(x, tokens, top, entropy, inv_t, ignore_index, True)
+        ctx.save_for_backward(x2, t, lse, h)
+        ctx.args = (inv_t, ignore_index, x.shape)
+        ctx.set_materialize_grads(False)
         if top:
-            ctx.mark_non_differentiable(tlp, tok)
-        return lp, h, tlp, tok
+            ctx.mark_non_differentiable(*out[2:])
+        return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g_lp, g_h, g_tlp, g_tok):
-        from . import _backend
         x2, t, lse, h = ctx.saved_tensors
         inv_t, ignore_index, shape = ctx.args
         if g_lp is None and g_h is None:
@@ -77,7 +81,7 @@ def token_logprobs(logits, tokens=None, top=0, entropy=False, temperature=1.0, i
                   index first among equals; not differentiable
     logprobs and entropy are differentiable with respect to the logits.  -inf logits have probability 0; a row of nothing else has
     log probability -inf, entropy 0 and gradient 0; a NaN or +inf makes its row NaN."""
-    if not isinstance(logits, torch.Tensor) or logits.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+    if not isinstance(logits, torch.Tensor) or logits.dtype not in _FLOATS:
         raise MxqError("logits must be a float32, float16 or bfloat16 tensor")
     if logits.dim() == 0 or logits.shape[-1] == 0:
         raise MxqError("logits need at least one value along the last dimension")
@@ -90,4 +94,11 @@ def token_logprobs(logits, tokens=None, top=0, entropy=False, temperature=1.0, i
     if not 0 < temperature < float("inf"):
         raise MxqError("temperature must be positive and finite")
     args = (logits, tokens, int(top), bool(entropy), 1.0 / temperature, int(ignore_index))
-    return TokenLogprobs(*(call(TokenLogprobsFunction, *args) if logits.is_cuda else _host(*args)))
+    if not logits.is_cuda:
+        return TokenLogprobs(*_host(*args))
+    if logits.requires_grad and torch.is_grad_enabled():
+        return TokenLogprobs(*TokenLogprobsFunction.apply(*args))
+    if logits.requires_grad or logits.dim() != 2:
+        with torch.no_grad():
+            return TokenLogprobs(*_run(*args, False)[4])
+    return TokenLogprobs(*_run(*args, False)[4])

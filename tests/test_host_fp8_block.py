@@ -131,3 +131,9 @@ def test_c_entries_refuse_before_they_launch():
     assert L.mxq_fp8_linear_fwd(p, 0, 32, 0, p, 32, p, 1, 0, p, 0, None, 0, 4, 8, 32, p, 100, None) == BAD   # workspace too small
     assert L.mxq_fp8_linear_fwd(p, 0, 32, 0, p, 32, p, 1, 0, p, 0, None, 0, 4, 8, 32, p + 16, 1 << 20, None) == ALIGN
     assert L.mxq_sum_partials(p, -1, 4, p, 0, None) == BAD
+    big = 1 << 30
+    assert L.mxq_fp8_linear_fwd_train(p, 0, 32, p, 0, 32, 0, None, 0, p, 0, 1, 1, p, 10, p, big, 4, 8, 32, None) == BAD    # saved too small
+    assert L.mxq_fp8_linear_fwd_train(p, 0, 32, p, 0, 32, 0, None, 0, p, 0, 0, 1, None, 0, p, big, 4, 8, 32, None) == BAD
+    assert L.mxq_fp8_linear_fwd_train(p, 0, 32, p, 0, 32, 0, None, 0, p, 0, 1, 1, p + 16, big, p, big, 4, 8, 32, None) == ALIGN
+    assert L.mxq_fp8_linear_bwd(p, 0, 8, 0, 0, p, big, 0, 1, p, 0, p, 0, None, 0, p, big, 4, 8, 32, None) == BAD           # dx, nothing saved
+    assert L.mxq_fp8_linear_bwd(p, 0, 8, 0, 0, p, big, 1, 1, p, 0, p, 0, None, 0, p, 10, 4, 8, 32, None) == BAD

@@ -76,7 +76,8 @@ def test_c_entries_refuse_before_they_launch():
     assert L.mxq_layer_norm_fwd(p, 2, 31, p, p, 2, p, p, p, 4, 32, 1e-5, None) == BAD             # rows overlap
     assert L.mxq_layer_norm_fwd(p, 2, 32, p, p, 1, p, p, p, 4, 32, 1e-5, None) == UNSUPPORTED     # bf16 with fp16 weights
     assert L.mxq_layer_norm_fwd(p, 2, 32, p, p, 2, p, p, p, 0, 32, 1e-5, None) == 0
-    assert L.mxq_layer_norm_bwd(p, p, 2, 32, 32, p, 2, None, p, p, p, 4, 32, None) == BAD
+    assert L.mxq_layer_norm_bwd(p, p, 2, 32, 32, p, 2, None, p, p, None, None, 2, None, 0, 4, 32, None) == BAD     # no statistics
+    assert L.mxq_layer_norm_bwd(p, p, 2, 32, 32, p, 2, p, p, p, p, None, 2, p, 8, 4, 32, None) == BAD       # workspace too small
     assert L.mxq_token_logprobs(p, 2, 32, p, -100, 1.0, p, None, None, 33, p, p, 4, 64, None) == LARGE
     assert L.mxq_token_logprobs(p, 2, 64, p, -100, 1.0, p, None, None, 3, None, p, 4, 64, None) == BAD
     assert L.mxq_token_logprobs(p, 2, 64, p, -100, 0.0, p, None, None, 0, None, None, 4, 64, None) == BAD
