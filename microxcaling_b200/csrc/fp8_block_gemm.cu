@@ -47,6 +47,34 @@ __device__ __forceinline__ void store_dyn(void* p, int dtype, int64_t i, float v
     else store1<DT_BF16>(p, i, v);
 }
 
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, int dtype) {
+    if (dtype == DT_BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// four consecutive values of an output row, bias added; `whole`: rows are a multiple of four values long
+__device__ __forceinline__ void store4(const Fp8Gemm& g, int64_t row, int64_t p, float4 f, bool whole) {
+    float v[4] = {f.x, f.y, f.z, f.w};
+    if (g.bias) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (p + j < g.P) v[j] += load_dyn(g.bias, g.bias_dtype, p + j);
+    }
+    if (!whole) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (p + j < g.P) store_dyn(g.out, g.out_dtype, row + p + j, v[j]);
+    } else if (g.out_dtype == DT_F32) {
+        *reinterpret_cast<float4*>(reinterpret_cast<float*>(g.out) + row + p) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+        *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(g.out) + row + p) =
+            make_uint2(pack2(v[0], v[1], g.out_dtype), pack2(v[2], v[3], g.out_dtype));
+    }
+}
+
 template <int NT>
 struct Fp8Tile {
     static constexpr int kWarps = NT >= 64 ? 8 : 4;           // epilogue warps: a lane quarter each, or half of its columns
@@ -181,22 +209,29 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
     }
     __syncthreads();
     if (g.split > 1) { ptx::cluster_arrive(); ptx::cluster_wait(); }
-    // each CTA of the cluster joins and writes its share of the tile's columns (output rows)
+    // each CTA of the cluster joins and writes its share of the tile's columns (output rows), four values a thread; the
+    // reads of the other CTAs' memory are issued together, their latency is what this phase costs
     if (!*abort_flag) {
         const int q_first = NT * rank / g.split, q_last = NT * (rank + 1) / g.split;
-        for (int i = q_first * 128 + threadIdx.x; i < q_last * 128; i += S::kThreads) {
+        const bool whole = g.P % 4 == 0;
+        for (int i = q_first * 128 + threadIdx.x * 4; i < q_last * 128; i += S::kThreads * 4) {
             const int64_t q = qt * NT + (i >> 7), p = pt * 128 + (i & 127);
             if (q >= g.Q) break;
             if (p >= g.P) continue;
-            float v = 0.f;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             if (g.split > 1) {
                 const uint32_t a = ptx::smem_u32(sums + i);
-                for (int r = 0; r < g.split; ++r) v += ptx::ld_cluster_f32(ptx::mapa(a, r));
+                float4 part[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (r < g.split) part[r] = ptx::ld_cluster_f32x4(ptx::mapa(a, r));
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (r < g.split) { v.x += part[r].x; v.y += part[r].y; v.z += part[r].z; v.w += part[r].w; }
             } else {
-                v = sums[i];
+                v = *reinterpret_cast<const float4*>(sums + i);
             }
-            if (g.bias) v += load_dyn(g.bias, g.bias_dtype, p);
-            store_dyn(g.out, g.out_dtype, q * g.P + p, v);
+            store4(g, q * g.P, p, v, whole);
         }
     }
     ptx::tc_fence_before();
@@ -206,6 +241,266 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
     if (warp == 1) {
         ptx::tc_fence_after();
         ptx::tmem_dealloc(tmem_base, S::kTmemCols);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Large products: CTA pairs (cta_group::2) on 256 x 256 tiles, persistent.  The tensor core's rows are a's here.  Each CTA
+// stages its own 128 rows of a and its half of b's 256 rows (32 KB a K block, five of them in flight), the even CTA issues the
+// MMAs for both, and every CTA's eight epilogue warps hold 128 x 256 fp32 sums in registers, 128 columns of a row a thread.
+// The two accumulators of 256 columns fill tensor memory: while the warps scale and add one block's sums the tensor core
+// works on the next one.  What has to fit beside its 512 cycles a block (128 x 256 x 128 at the peak rate on each SM) is
+// 32768 fused multiply-adds, 256 cycles of the fp32 pipes, and the 64 cycles in which the block leaves tensor memory;
+// with a scale for every row of b as well (B_ROWS: weight gradients) there is a second multiplication, and the fp32 pipes become the limit.
+// ---------------------------------------------------------------------------------------------------------------
+struct Fp8Pair {
+    const float* sa;
+    const float* sb;
+    int64_t sa_ld, sb_ld;
+    int sa_shift, sb_shift;
+    void* out;                                     // [M, N]
+    const void* bias;                              // [N] or null
+    int out_dtype, bias_dtype, tma_out;
+    int64_t M, N, kb_total, m_tiles, n_tiles;
+    uint32_t idesc;
+};
+
+template <bool B_ROWS>
+struct Fp8PairSmem {
+    static constexpr int kStages = 5;
+    static constexpr int kBoxes = B_ROWS ? 1 : 2;              // b's scales leave no room for a second one
+    static constexpr int kA = 128 * 128, kStage = 2 * kA;
+    static constexpr int kStgOff = kStages * kStage;           // boxes of 32 rows x 128 bytes for each epilogue warp
+    static constexpr int kScaleOff = kStgOff + 8 * kBoxes * 4096;       // b's scales of two blocks
+    static constexpr int kBarOff = kScaleOff + (B_ROWS ? 2 * 256 * 4 : 0);
+    static constexpr int kTotal = kBarOff + 256 + 1024;
+    static_assert(kTotal <= 232448, "shared memory");
+};
+
+// Tiles are walked in groups of 16 tile rows, column by column, so that CTAs at work at the same time share panels in L2.
+__device__ __forceinline__ void pair_tile(int64_t t, const Fp8Pair& g, int64_t& mt, int64_t& nt) {
+    const uint32_t per = 16 * (uint32_t)g.n_tiles, grp = (uint32_t)t / per, i = (uint32_t)t % per;
+    const uint32_t rows = min(16u, (uint32_t)g.m_tiles - grp * 16);
+    mt = grp * 16 + i % rows;
+    nt = i / rows;
+}
+
+// acc += (two sums of a block) * (their scales)
+__device__ __forceinline__ void scale_add(float2& acc, uint32_t lo, uint32_t hi, uint64_t scale) {
+    uint64_t x = ptx::pack2f(acc.x, acc.y);
+    ptx::fma2(x, ptx::pack2f(lo, hi), scale);
+    ptx::unpack2f(x, acc.x, acc.y);
+}
+
+template <bool B_ROWS, bool F32>
+__global__ void __launch_bounds__(384, 1)
+fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                     const __grid_constant__ CUtensorMap tmap_c, const Fp8Pair g) {
+    using S = Fp8PairSmem<B_ROWS>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBarOff);    // [kStages], the even CTA's
+    uint64_t* empty = full + S::kStages;                                // [kStages], one in each CTA
+    uint64_t* acc_full = empty + S::kStages;                            // [2], one in each CTA
+    uint64_t* acc_empty = acc_full + 2;                                 // [2], the even CTA's
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    float* b_scale = reinterpret_cast<float*>(smem + S::kScaleOff);     // [2][256]
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = ptx::cluster_ctarank();
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::kStages; ++s) { ptx::mbar_init(ptx::smem_u32(&full[s]), 1); ptx::mbar_init(ptx::smem_u32(&empty[s]), 1); }
+        for (int b = 0; b < 2; ++b) { ptx::mbar_init(ptx::smem_u32(&acc_full[b]), 1); ptx::mbar_init(ptx::smem_u32(&acc_empty[b]), 16); }
+        *abort_flag = 0;
+        ptx::fence_mbar_init();
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc_pair(ptx::smem_u32(tmem_slot), 512);
+        ptx::tmem_relinquish_pair();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::cluster_arrive();                                    // both CTAs' barriers exist before anyone signals them
+    ptx::cluster_wait();
+    ptx::tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int64_t total = g.m_tiles * g.n_tiles, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+    // Registers: 384 threads are launched with 168 each (64512); the first warpgroup (producer, MMA issuer, two idle warps)
+    // keeps 40 and the epilogue's two take 232 each, 64512 in all.
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (warp == 0 && ptx::elect_one()) {
+            ptx::prefetch_tmap(&tmap_a);
+            ptx::prefetch_tmap(&tmap_b);
+            uint32_t it = 0;
+            bool ok = true;
+            for (int64_t t = pair; t < total && ok; t += pairs) {
+                int64_t mt, nt;
+                pair_tile(t, g, mt, nt);
+                const int row_a = (int)(mt * 256 + rank * 128), row_b = (int)(nt * 256 + rank * 128);
+                for (int64_t kb = 0; kb < g.kb_total; ++kb, ++it) {
+                    const int s = it % S::kStages;
+                    if (it >= (uint32_t)S::kStages && !ptx::mbar_wait(ptx::smem_u32(&empty[s]), ((it / S::kStages) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                    if (rank == 0) ptx::mbar_expect_tx(ptx::smem_u32(&full[s]), 2 * S::kStage);
+                    const uint32_t bar = ptx::mapa(ptx::smem_u32(&full[s]), 0), st = ptx::smem_u32(smem + s * S::kStage);
+                    ptx::tma_load_2d_pair(st, &tmap_a, bar, (int)(kb * 128), row_a);
+                    ptx::tma_load_2d_pair(st + S::kA, &tmap_b, bar, (int)(kb * 128), row_b);
+                }
+            }
+        }
+        if (warp == 1 && rank == 0 && ptx::elect_one()) {
+            const uint64_t desc = ptx::smem_desc(ptx::smem_u32(smem), 0, 1024, 2);
+            uint32_t it = 0;
+            bool ok = true;
+            for (int64_t t = pair; t < total && ok; t += pairs) {
+                for (int64_t kb = 0; kb < g.kb_total; ++kb, ++it) {
+                    const int s = it % S::kStages;
+                    const uint32_t b = it & 1;
+                    if (!ptx::mbar_wait(ptx::smem_u32(&full[s]), (it / S::kStages) & 1, abort_flag)) { ok = false; break; }
+                    const uint64_t ad = desc + (uint64_t)((s * S::kStage) >> 4), bd = ad + (S::kA >> 4);
+                    if (it >= 2 && !ptx::mbar_wait(ptx::smem_u32(&acc_empty[b]), ((it >> 1) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                    ptx::tc_fence_after();
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)                // 32 bytes further inside the swizzle atom a step
+                        ptx::tc_mma_f8_pair(tmem_base + b * 256, ad + 2 * k, bd + 2 * k, g.idesc, k > 0);
+                    ptx::tc_commit_pair(ptx::smem_u32(&acc_full[b]), 3);
+                    ptx::tc_commit_pair(ptx::smem_u32(&empty[s]), 3);
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        const int e = warp - 4, quarter = warp & 3, half = e >> 2;
+        const int te = threadIdx.x & 127;                     // one of the 128 threads of this half
+        const uint32_t boxes = S::kStgOff + e * (S::kBoxes * 4096);
+        uint32_t ring = 0;
+        uint32_t it = 0;
+        bool ok = true;
+        // the scales of the next block are fetched a block ahead
+        int64_t mt = 0, nt = 0;
+        float sa_next = 0.f, sb_next = 0.f;
+        const float *sap = nullptr, *sbp = nullptr;
+        auto aim = [&](int64_t t) {
+            pair_tile(t, g, mt, nt);
+            const int64_t row = mt * 256 + rank * 128 + quarter * 32 + lane;
+            sap = g.sa + (min(row, g.M - 1) >> g.sa_shift);
+            const int64_t col = nt * 256 + half * 128 + (B_ROWS ? te : 0);
+            sbp = g.sb + (min(col, g.N - 1) >> g.sb_shift);
+            sa_next = __ldg(sap);
+            sb_next = __ldg(sbp);
+        };
+        if (pair < total) aim(pair);
+        for (int64_t t = pair; t < total && ok; t += pairs) {
+            const int64_t row0 = mt * 256 + rank * 128 + quarter * 32, col0 = nt * 256 + half * 128;
+            float2 acc[64];                                  // pairs of columns
+#pragma unroll
+            for (int i = 0; i < 64; ++i) acc[i] = make_float2(0.f, 0.f);
+            for (int64_t kb = 0; kb < g.kb_total; ++kb, ++it) {
+                const uint32_t b = it & 1;
+                const float sa = sa_next;
+                const uint64_t f = B_ROWS ? ptx::pack2f(sa, sa) : ptx::pack2f(sa * sb_next, sa * sb_next);
+                const float* bs = b_scale + b * 256 + half * 128;
+                if constexpr (B_ROWS) b_scale[b * 256 + half * 128 + te] = sb_next;
+                if (kb + 1 < g.kb_total) {
+                    sa_next = __ldg(sap += g.sa_ld);
+                    sb_next = __ldg(sbp += g.sb_ld);
+                }
+                if constexpr (B_ROWS) asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");   // two buffers: a warp is at most one block ahead
+                if (!ptx::mbar_wait(ptx::smem_u32(&acc_full[b]), (it >> 1) & 1, abort_flag)) {
+                    ok = false;                                // counts the blocks to the end all the same: every later wait gives up at once
+                }
+                ptx::tc_fence_after();
+                const uint32_t ta = tmem_base + ((uint32_t)(quarter * 32) << 16) + b * 256 + half * 128;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t w[64];
+                    ptx::tmem_ld_32x32b_x32(ta + 64 * c, w);
+                    ptx::tmem_ld_32x32b_x32(ta + 64 * c + 32, w + 32);
+                    ptx::tmem_ld_wait();
+                    if (c == 1) {                              // the accumulator is out of tensor memory
+                        ptx::tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) ptx::mbar_arrive_cluster_tmem(ptx::mapa(ptx::smem_u32(&acc_empty[b]), 0));
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        uint64_t m0 = f, m1 = f;
+                        if constexpr (B_ROWS) {
+                            const float4 q = *reinterpret_cast<const float4*>(bs + 64 * c + 2 * i);
+                            m0 = ptx::mul2(f, ptx::pack2f(q.x, q.y));
+                            m1 = ptx::mul2(f, ptx::pack2f(q.z, q.w));
+                        }
+                        scale_add(acc[32 * c + i], w[2 * i], w[2 * i + 1], m0);
+                        scale_add(acc[32 * c + i + 1], w[2 * i + 2], w[2 * i + 3], m1);
+                    }
+                }
+            }
+            if (t + pairs < total) aim(t + pairs);
+            if (!ok || row0 >= g.M || col0 >= g.N) continue;
+            if (g.bias) {
+#pragma unroll
+                for (int i = 0; i < 64; ++i) {
+                    acc[i].x += load_dyn(g.bias, g.bias_dtype, min(col0 + 2 * i, g.N - 1));
+                    acc[i].y += load_dyn(g.bias, g.bias_dtype, min(col0 + 2 * i + 1, g.N - 1));
+                }
+            }
+            // out through boxes of 32 rows x 128 bytes in the 128-byte swizzle of the output's tensor map
+            constexpr int PER = F32 ? 32 : 64;                 // columns of a box
+#pragma unroll
+            for (int c = 0; c < 128 / PER; ++c) {
+                const int64_t col = col0 + PER * c;
+                if (col >= g.N) break;
+                uint8_t* box = smem + boxes + (ring++ % S::kBoxes) * 4096;
+                if (lane == 0) ptx::bulk_wait_read<S::kBoxes - 1>();       // this box's last store has read it
+                __syncwarp();
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if constexpr (F32) {
+                            const float2 p = acc[16 * c + 2 * q + (j >> 1)];
+                            w[j] = __float_as_uint(j & 1 ? p.y : p.x);
+                        } else {
+                            const float2 p = acc[32 * c + 4 * q + j];
+                            w[j] = pack2(p.x, p.y, g.out_dtype);
+                        }
+                    }
+                    ptx::st_shared_v4(ptx::smem_u32(box) + lane * 128 + ((q ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
+                }
+                if (g.tma_out) {
+                    ptx::fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) { ptx::tma_store_2d(&tmap_c, ptx::smem_u32(box), (int)col, (int)row0); ptx::bulk_commit(); }
+                } else {                                       // rows that are no multiple of 16 bytes long
+                    __syncwarp();
+                    const int n = (int)min((int64_t)32, g.M - row0);
+                    for (int r = 0; r < n; ++r) {
+                        const uint32_t v = *reinterpret_cast<const uint32_t*>(box + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+                        const int64_t at = (row0 + r) * g.N + col;
+                        if constexpr (F32) {
+                            if (col + lane < g.N) reinterpret_cast<uint32_t*>(g.out)[at + lane] = v;
+                        } else {
+                            if (col + 2 * lane < g.N) reinterpret_cast<uint16_t*>(g.out)[at + 2 * lane] = (uint16_t)v;
+                            if (col + 2 * lane + 1 < g.N) reinterpret_cast<uint16_t*>(g.out)[at + 2 * lane + 1] = (uint16_t)(v >> 16);
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+        if (lane == 0) ptx::bulk_wait_all();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::cluster_arrive();                                    // the partner no longer touches this CTA's memory
+    ptx::cluster_wait();
+    if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_fp8_status, MXQ_ERR_DEVICE);
+    if (warp == 1) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc_pair(tmem_base, 512);
     }
 }
 
@@ -244,6 +539,38 @@ static int launch_fp8(const CUtensorMap& tp, const CUtensorMap& tq, const Fp8Gem
     return check_launch();
 }
 
+// out [M, N]: boxes of 32 rows x 128 bytes
+static int make_out_map(CUtensorMap* m, void* base, int64_t M, int64_t N, int dtype) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return MXQ_ERR_CUDA;
+    const cuuint64_t es = (cuuint64_t)dtype_size(dtype);
+    cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)M};
+    cuuint64_t strides[1] = {(cuuint64_t)N * es};
+    cuuint32_t box[2] = {(cuuint32_t)(128 / es), 32};
+    cuuint32_t estr[2] = {1, 1};
+    const CUtensorMapDataType t = dtype == MXQ_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
+    return fn(m, t, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? MXQ_OK : MXQ_ERR_CUDA;
+}
+
+template <bool B_ROWS, bool F32>
+static int launch_fp8_pair(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const Fp8Pair& g, cudaStream_t st) {
+    auto kern = fp8_gemm_pair_kernel<B_ROWS, F32>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Fp8PairSmem<B_ROWS>::kTotal) != cudaSuccess) { cudaGetLastError(); return MXQ_ERR_CUDA; }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * (unsigned)std::min<int64_t>(g.m_tiles * g.n_tiles, std::max(gemm_sms() / 2, 1)));
+    cfg.blockDim = dim3(384);
+    cfg.dynamicSmemBytes = Fp8PairSmem<B_ROWS>::kTotal;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kern, ta, tb, tc, g) != cudaSuccess) { cudaGetLastError(); return MXQ_ERR_CUDA; }
+    return check_launch();
+}
+
 int fp8_gemm_status(int clear) {
     int v = 0;
     if (cudaMemcpyFromSymbol(&v, g_fp8_status, sizeof v) != cudaSuccess) { cudaGetLastError(); return MXQ_ERR_CUDA; }
@@ -266,6 +593,27 @@ extern "C" int mxq_fp8_gemm(const void* a, int64_t a_pitch, const float* a_scale
     if (!a || !b || !a_scales || !b_scales || !out || a_pitch < K || b_pitch < K) return MXQ_ERR_BAD_ARG;
     if (!aligned16(a) || !aligned16(b) || a_pitch % 16 || b_pitch % 16) return MXQ_ERR_ALIGN;
     if (M > 0x7fffff00 || N > 0x7fffff00 || K > 0x7fffff00) return MXQ_ERR_TOO_LARGE;
+    cudaStream_t st = (cudaStream_t)stream;
+    const int64_t tiles2 = ((M + 255) / 256) * ((N + 255) / 256);
+    if (M >= 256 && N >= 256 && tiles2 >= sm_count() / 4) {                                // pairs of CTAs where at least half of the pairs have a tile
+        Fp8Pair g;
+        g.sa = a_scales; g.sa_shift = a_tile ? 7 : 0; g.sa_ld = a_tile ? (M + 127) / 128 : M;
+        g.sb = b_scales; g.sb_shift = b_tile ? 7 : 0; g.sb_ld = b_tile ? (N + 127) / 128 : N;
+        g.out = out; g.out_dtype = out_dtype; g.bias = bias; g.bias_dtype = bias_dtype;
+        g.M = M; g.N = N; g.kb_total = (K + 127) / 128;
+        g.m_tiles = (M + 255) / 256; g.n_tiles = (N + 255) / 256;
+        g.idesc = ptx::idesc_f8(a_fmt, b_fmt, 256, 256);
+        g.tma_out = aligned16(out) && (N * dtype_size(out_dtype)) % 16 == 0;
+        CUtensorMap ta, tb, tc;
+        int rc = make_map(&ta, a, M, K, a_pitch, 128);
+        if (!rc) rc = make_map(&tb, b, N, K, b_pitch, 128);
+        tc = ta;
+        if (!rc && g.tma_out) rc = make_out_map(&tc, out, M, N, out_dtype);
+        if (rc) return rc;
+        g_launch_count[0].fetch_add(1, std::memory_order_relaxed);
+        if (out_dtype == MXQ_F32) return g.sb_shift ? launch_fp8_pair<false, true>(ta, tb, tc, g, st) : launch_fp8_pair<true, true>(ta, tb, tc, g, st);
+        return g.sb_shift ? launch_fp8_pair<false, false>(ta, tb, tc, g, st) : launch_fp8_pair<true, false>(ta, tb, tc, g, st);
+    }
     const int nt = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
     Fp8Gemm g;
     g.sp = b_scales; g.sp_shift = b_tile ? 7 : 0; g.sp_ld = b_tile ? (N + 127) / 128 : N;
@@ -282,7 +630,6 @@ extern "C" int mxq_fp8_gemm(const void* a, int64_t a_pitch, const float* a_scale
     if (!rc) rc = make_map(&tq, a, M, K, a_pitch, nt);
     if (rc) return rc;
     g_launch_count[0].fetch_add(1, std::memory_order_relaxed);
-    cudaStream_t st = (cudaStream_t)stream;
     if (nt == 16) return launch_fp8<16>(tp, tq, g, st);
     if (nt == 32) return launch_fp8<32>(tp, tq, g, st);
     if (nt == 64) return launch_fp8<64>(tp, tq, g, st);

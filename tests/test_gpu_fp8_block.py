@@ -84,7 +84,8 @@ def test_quantize_strides_and_leading_dimensions(mx):
 
 
 PRODUCTS = [(1, 1, 1), (1, 4096, 4096), (3, 130, 100), (16, 128, 128), (17, 300, 512), (33, 1, 2000), (64, 256, 1024), (65, 129, 4097),
-            (128, 128, 256), (200, 1000, 1511), (300, 520, 640), (777, 1032, 1160), (1024, 1024, 2048)]
+            (128, 128, 256), (200, 1000, 1511), (300, 520, 640), (777, 1032, 1160), (1024, 1024, 2048),
+            (2050, 2304, 1100), (1500, 2311, 384), (9500, 200, 130), (300, 5000, 1)]   # enough 256 x 256 tiles for CTA pairs
 
 
 @pytest.mark.parametrize("shape", PRODUCTS)
