@@ -422,7 +422,7 @@ int mxq_sum_partials(const float* part, int64_t n, int64_t cols, void* out, int 
 /*
  * out[m, n] = sum over 128-blocks kb of K of sa[kb, m] * sb[kb, n] * (sum over k in kb of a[m, k] * b[n, k]) (+ bias[n]),
  * rounded once to out_dtype.  a [M, K], b [N, K]: operands as mxq_fp8_quantize writes them (`*_fmt` 0 e4m3, 1 e5m2;
- * `*_tile`: scales of 128 x 128 blocks); out [M, N] contiguous; bias [N] of bias_dtype, or NULL.  The product of two scales
+ * `*_tile`: scales of 128 x 128 blocks); out [M, N] contiguous, 16-byte aligned; bias [N] of bias_dtype, or NULL.  The product of two scales
  * has to be representable in fp32.  Sums are fp32; results do not depend on timing.  K > 0.
  */
 int mxq_fp8_gemm(const void* a, int64_t a_pitch, const float* a_scales, int a_tile, int a_fmt, const void* b,

@@ -10,9 +10,10 @@
 // The tensor core's 128 rows are taken from b, so that the 32 lanes of an epilogue warp hold 32 consecutive n
 // of one output row and a product with few rows (tokens of a decoding step) wastes nothing: a tile is 128 of b's rows
 // x NT of a's rows, NT = 16 .. 128, and what has to be read then is b, once.  When the tiles do not fill the GPU the K blocks
-// of a tile are split over the CTAs of a cluster (2, 4 or 8), which join their sums through distributed shared
-// memory in the order of their ranks, so that results do not depend on timing.
+// of a tile are split over the CTAs of a cluster (2, 4 or 8): each sends its sums to the CTA that owns those output rows, through
+// distributed shared memory, and the owner adds them in the order of the ranks, so that results do not depend on timing.
 #include <cuda.h>
+#include <math.h>
 #include <algorithm>
 #include "fp8_block.cuh"
 #include "mxq_common.cuh"
@@ -33,6 +34,7 @@ struct Fp8Gemm {
     int out_dtype, bias_dtype;
     int64_t P, Q, kb_total, p_tiles, q_tiles;
     int split;                                     // CTAs of a cluster that share a tile
+    int early;                                     // launched while the kernel that writes a's operand may still run
     uint32_t idesc;
 };
 
@@ -75,7 +77,7 @@ __device__ __forceinline__ void store4(const Fp8Gemm& g, int64_t row, int64_t p,
     }
 }
 
-template <int NT>
+template <int NT, bool SPLIT>
 struct Fp8Tile {
     static constexpr int kWarps = NT >= 64 ? 8 : 4;           // epilogue warps: a lane quarter each, or half of its columns
     static constexpr int kCols = NT >= 64 ? NT / 2 : NT;      // columns of one epilogue warp
@@ -84,17 +86,20 @@ struct Fp8Tile {
     static constexpr int kTmemCols = kAcc * NT < 32 ? 32 : kAcc * NT;
     static constexpr int kP = 128 * 128, kQ = NT * 128;
     static constexpr int kStage = kP + kQ;
-    static constexpr int kStages = NT >= 128 ? 6 : NT == 64 ? 4 : 5;
-    static constexpr int kSum = NT * 128 * 4;                 // this CTA's sums, over the stages once they are done with
-    static constexpr int kScaleOff = kStages * kStage > kSum ? kStages * kStage : kSum;
+    // As many stages as let two CTAs live on an SM (one with NT = 128).  Sums from other CTAs need memory of their own, beside
+    // the stages that may still be in use; a CTA that has the tile to itself passes its sums through the stages.
+    static constexpr int kStages = NT == 128 ? (SPLIT ? 4 : 6) : NT == 64 ? (SPLIT ? 3 : 4) : NT == 32 ? (SPLIT ? 4 : 5) : (SPLIT ? 5 : 6);
+    static constexpr int kJoinOff = SPLIT ? kStages * kStage : 0;   // [rank][own columns][128] sums sent to this CTA
+    static constexpr int kScaleOff = kStages * kStage + (SPLIT ? NT * 128 * 4 : 0);
+    static_assert(NT * 128 * 4 <= kStages * kStage, "the sums fit into the stages");
     static constexpr int kBarOff = kScaleOff + 2 * NT * 4;
     static constexpr int kTotal = kBarOff + 256 + 1024;
 };
 
-template <int NT>
-__global__ void __launch_bounds__(Fp8Tile<NT>::kThreads)
+template <int NT, bool SPLIT>
+__global__ void __launch_bounds__(Fp8Tile<NT, SPLIT>::kThreads)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ CUtensorMap tmap_q, const Fp8Gemm g) {
-    using S = Fp8Tile<NT>;
+    using S = Fp8Tile<NT, SPLIT>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBarOff);    // [kStages]
@@ -104,52 +109,68 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + S::kAcc);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     float* q_scale = reinterpret_cast<float*>(smem + S::kScaleOff);     // [2][NT]
-    float* sums = reinterpret_cast<float*>(smem);                       // [NT][128], after the main loop
+    float* join = reinterpret_cast<float*>(smem + S::kJoinOff);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = g.split > 1 ? (int)ptx::cluster_ctarank() : 0;
-    const int64_t tile = blockIdx.x / g.split;
-    const int64_t pt = tile % g.p_tiles, qt = tile / g.p_tiles;
-    const int64_t kb0 = g.kb_total * rank / g.split, kb1 = g.kb_total * (rank + 1) / g.split;
+    const int rank = SPLIT ? (int)ptx::cluster_ctarank() : 0;
+    const uint32_t tile = blockIdx.x / g.split;
+    const int64_t pt = tile / (uint32_t)g.q_tiles, qt = tile % (uint32_t)g.q_tiles;   // tiles that share rows of b side by side
+    const int blocks = (int)g.kb_total, kb0 = blocks * rank / g.split, n_kb = blocks * (rank + 1) / g.split - kb0;
 
-    if (threadIdx.x == 0) {
+    // The producer's thread makes the barriers and sends for the first stages before anyone else is ready.
+    const bool producer = warp == 0 && ptx::elect_one();
+    auto load_p = [&](int i) {
+        const int s = i % S::kStages;
+        const uint32_t bar = ptx::smem_u32(&full[s]);
+        ptx::mbar_expect_tx(bar, S::kStage);
+        ptx::tma_load_2d(ptx::smem_u32(smem + s * S::kStage), &tmap_p, bar, (kb0 + i) * 128, (int)(pt * 128));
+    };
+    auto load_q = [&](int i) {
+        const int s = i % S::kStages;
+        ptx::tma_load_2d(ptx::smem_u32(smem + s * S::kStage + S::kP), &tmap_q, ptx::smem_u32(&full[s]), (kb0 + i) * 128, (int)(qt * NT));
+    };
+    if (producer) {
         for (int s = 0; s < S::kStages; ++s) { ptx::mbar_init(ptx::smem_u32(&full[s]), 1); ptx::mbar_init(ptx::smem_u32(&empty[s]), 1); }
         for (int b = 0; b < S::kAcc; ++b) { ptx::mbar_init(ptx::smem_u32(&acc_full[b]), 1); ptx::mbar_init(ptx::smem_u32(&acc_empty[b]), S::kWarps); }
         *abort_flag = 0;
         ptx::fence_mbar_init();
+        ptx::fence_proxy_async();
+        const int ahead = min((int)S::kStages, n_kb);
+        for (int i = 0; i < ahead; ++i) load_p(i);
+        if (g.early) ptx::grid_wait();                        // b was there before the kernel in front of this one began, a was not
+        for (int i = 0; i < ahead; ++i) load_q(i);
     }
     if (warp == 1) {
         ptx::tmem_alloc(ptx::smem_u32(tmem_slot), S::kTmemCols);
         ptx::tmem_relinquish();
     }
+    __syncwarp();
     ptx::tc_fence_before();
     __syncthreads();
+    if constexpr (SPLIT) ptx::cluster_arrive();                   // waited for before the first store to another CTA's memory
     ptx::tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
     if (warp == 0) {
-        if (ptx::elect_one()) {
-            uint32_t it = 0;
+        if (producer) {
             bool ok = true;
-            for (int64_t kb = kb0; kb < kb1; ++kb, ++it) {
-                const int s = it % S::kStages;
-                if (it >= (uint32_t)S::kStages && !ptx::mbar_wait(ptx::smem_u32(&empty[s]), ((it / S::kStages) & 1) ^ 1, abort_flag)) { ok = false; break; }
-                const uint32_t bar = ptx::smem_u32(&full[s]), st = ptx::smem_u32(smem + s * S::kStage);
-                ptx::mbar_expect_tx(bar, S::kStage);
-                ptx::tma_load_2d(st, &tmap_p, bar, (int)(kb * 128), (int)(pt * 128));
-                ptx::tma_load_2d(st + S::kP, &tmap_q, bar, (int)(kb * 128), (int)(qt * NT));
+            for (int i = S::kStages; i < n_kb; ++i) {
+                if (!ptx::mbar_wait(ptx::smem_u32(&empty[i % S::kStages]), ((i / S::kStages) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                load_p(i);
+                load_q(i);
             }
             if (!ok)                               // give copies already in flight a bounded time to land
                 for (int s = 0; s < S::kStages; ++s)
                     for (uint32_t i = 0; i < 4096 && !ptx::mbar_try_wait(ptx::smem_u32(&full[s]), 0) &&
                                          !ptx::mbar_try_wait(ptx::smem_u32(&full[s]), 1); ++i) __nanosleep(64);
         }
+        __syncwarp();
+        if constexpr (SPLIT) ptx::cluster_wait();
     } else if (warp == 1) {
         if (ptx::elect_one()) {
-            uint32_t it = 0;
-            for (int64_t kb = kb0; kb < kb1; ++kb, ++it) {
+            for (int it = 0; it < n_kb; ++it) {
                 const int s = it % S::kStages, b = it % S::kAcc;
-                if (it >= (uint32_t)S::kAcc && !ptx::mbar_wait(ptx::smem_u32(&acc_empty[b]), ((it / S::kAcc) & 1) ^ 1, abort_flag)) break;
+                if (it >= S::kAcc && !ptx::mbar_wait(ptx::smem_u32(&acc_empty[b]), ((it / S::kAcc) & 1) ^ 1, abort_flag)) break;
                 if (!ptx::mbar_wait(ptx::smem_u32(&full[s]), (it / S::kStages) & 1, abort_flag)) break;
                 ptx::tc_fence_after();
                 const uint32_t pa = ptx::smem_u32(smem + s * S::kStage), qa = pa + S::kP;
@@ -161,33 +182,35 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
                 ptx::tc_commit(ptx::smem_u32(&acc_full[b]));
             }
         }
+        __syncwarp();
+        if constexpr (SPLIT) ptx::cluster_wait();
     } else {
         const int e = warp - 2, quarter = warp & 3, c0 = NT >= 64 ? (e >> 2) * S::kCols : 0;
         const int te = threadIdx.x - 64;                       // 0 .. 32 * kWarps - 1
         const int64_t p = pt * 128 + quarter * 32 + lane;
-        const float* spp = g.sp + (min(p, g.P - 1) >> g.sp_shift);
+        const float* spp = g.sp + (min(p, g.P - 1) >> g.sp_shift) + kb0 * g.sp_ld;
         const bool loads_q = te < NT && qt * NT + te < g.Q;
-        const float* sqp = g.sq + ((qt * NT + te) >> g.sq_shift);
+        const float* sqp = g.sq + ((qt * NT + te) >> g.sq_shift) + kb0 * g.sq_ld;
         float acc[S::kCols];
 #pragma unroll
         for (int i = 0; i < S::kCols; ++i) acc[i] = 0.f;
         float sp_next = 0.f, sq_next = 0.f;
-        if (kb0 < kb1) {
-            sp_next = __ldg(spp + kb0 * g.sp_ld);
-            if (loads_q) sq_next = __ldg(sqp + kb0 * g.sq_ld);
+        if (g.early) ptx::grid_wait();                         // a's scales; and the output may not be written before
+        if (n_kb > 0) {
+            sp_next = __ldg(spp);
+            if (loads_q) sq_next = __ldg(sqp);
         }
-        uint32_t it = 0;
-        for (int64_t kb = kb0; kb < kb1; ++kb, ++it) {
+        for (int it = 0; it < n_kb; ++it) {
             const int b = it % S::kAcc;
             float* qs = q_scale + (it & 1) * NT;
             if (te < NT) qs[te] = sq_next;
             const float sp = sp_next;
-            if (kb + 1 < kb1) {
-                sp_next = __ldg(spp + (kb + 1) * g.sp_ld);
-                if (loads_q) sq_next = __ldg(sqp + (kb + 1) * g.sq_ld);
+            if (it + 1 < n_kb) {
+                sp_next = __ldg(spp += g.sp_ld);
+                if (loads_q) sq_next = __ldg(sqp += g.sq_ld);
             }
             asm volatile("bar.sync 1, %0;" ::"n"(32 * S::kWarps) : "memory");   // two buffers: a warp is at most one block ahead
-            if (!ptx::mbar_wait(ptx::smem_u32(&acc_full[b]), (it / S::kAcc) & 1, abort_flag)) *abort_flag = 1;
+            ptx::mbar_wait(ptx::smem_u32(&acc_full[b]), (it / S::kAcc) & 1, abort_flag);   // a wait that gives up raises the flag
             ptx::tc_fence_after();
             const uint32_t t = tmem_base + ((uint32_t)(quarter * 32) << 16) + b * NT + c0;
 #pragma unroll
@@ -195,48 +218,58 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
                 uint32_t v[16];
                 ptx::tmem_ld_32x32b_x16(t + c, v);
                 ptx::tmem_ld_wait();
+                if (c + 16 == S::kCols) {                      // the accumulator is out of tensor memory
+                    ptx::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&acc_empty[b]));
+                }
 #pragma unroll
-                for (int i = 0; i < 16; ++i) acc[c + i] = __fmaf_rn(__uint_as_float(v[i]), sp * qs[c0 + c + i], acc[c + i]);
+                for (int i = 0; i < 16; i += 4) {
+                    const float4 q = *reinterpret_cast<const float4*>(qs + c0 + c + i);
+                    acc[c + i] = __fmaf_rn(__uint_as_float(v[i]), sp * q.x, acc[c + i]);
+                    acc[c + i + 1] = __fmaf_rn(__uint_as_float(v[i + 1]), sp * q.y, acc[c + i + 1]);
+                    acc[c + i + 2] = __fmaf_rn(__uint_as_float(v[i + 2]), sp * q.z, acc[c + i + 2]);
+                    acc[c + i + 3] = __fmaf_rn(__uint_as_float(v[i + 3]), sp * q.w, acc[c + i + 3]);
+                }
             }
-            ptx::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&acc_empty[b]));
         }
-        // every block of this CTA has been multiplied and every copy has landed: the stages are free
-        asm volatile("bar.sync 1, %0;" ::"n"(32 * S::kWarps) : "memory");
+        // send the sums to the CTAs that own their columns (output rows): [rank][own column][128]
+        const int own = NT / g.split;                          // a power of two
+        const int shift = __ffs(own) - 1;
+        const uint32_t mine = ptx::smem_u32(join) + 4 * (rank * own * 128 + quarter * 32 + lane);
+        if constexpr (SPLIT) {
+            ptx::cluster_wait();                               // the other CTAs are there
 #pragma unroll
-        for (int i = 0; i < S::kCols; ++i) sums[(c0 + i) * 128 + quarter * 32 + lane] = acc[i];
+            for (int i = 0; i < S::kCols; ++i) {
+                const int c = c0 + i;
+                ptx::st_cluster_f32(ptx::mapa(mine, c >> shift) + (c & (own - 1)) * 512, acc[i]);
+            }
+        } else {
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * S::kWarps) : "memory");   // the last block has been multiplied: the stages are free
+#pragma unroll
+            for (int i = 0; i < S::kCols; ++i) join[(c0 + i) * 128 + quarter * 32 + lane] = acc[i];
+        }
     }
-    __syncthreads();
-    if (g.split > 1) { ptx::cluster_arrive(); ptx::cluster_wait(); }
-    // each CTA of the cluster joins and writes its share of the tile's columns (output rows), four values a thread; the
-    // reads of the other CTAs' memory are issued together, their latency is what this phase costs
+    if constexpr (SPLIT) { __syncwarp(); ptx::cluster_arrive(); ptx::cluster_wait(); }
+    else __syncthreads();
+    // join and write this CTA's columns, four consecutive values of an output row a thread
     if (!*abort_flag) {
-        const int q_first = NT * rank / g.split, q_last = NT * (rank + 1) / g.split;
+        const int own = NT / g.split;
         const bool whole = g.P % 4 == 0;
-        for (int i = q_first * 128 + threadIdx.x * 4; i < q_last * 128; i += S::kThreads * 4) {
-            const int64_t q = qt * NT + (i >> 7), p = pt * 128 + (i & 127);
+        for (int i = threadIdx.x * 4; i < own * 128; i += S::kThreads * 4) {
+            const int64_t q = qt * NT + rank * own + (i >> 7), p = pt * 128 + (i & 127);
             if (q >= g.Q) break;
             if (p >= g.P) continue;
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (g.split > 1) {
-                const uint32_t a = ptx::smem_u32(sums + i);
-                float4 part[8];
-#pragma unroll
-                for (int r = 0; r < 8; ++r)
-                    if (r < g.split) part[r] = ptx::ld_cluster_f32x4(ptx::mapa(a, r));
-#pragma unroll
-                for (int r = 0; r < 8; ++r)
-                    if (r < g.split) { v.x += part[r].x; v.y += part[r].y; v.z += part[r].z; v.w += part[r].w; }
-            } else {
-                v = *reinterpret_cast<const float4*>(sums + i);
+            float4 v = *reinterpret_cast<const float4*>(join + i);
+            for (int r = 1; r < g.split; ++r) {
+                const float4 o = *reinterpret_cast<const float4*>(join + r * own * 128 + i);
+                v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
             }
             store4(g, q * g.P, p, v, whole);
         }
     }
     ptx::tc_fence_before();
     __syncthreads();
-    if (g.split > 1) { ptx::cluster_arrive(); ptx::cluster_wait(); }       // no CTA leaves while another reads its sums
     if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_fp8_status, MXQ_ERR_DEVICE);
     if (warp == 1) {
         ptx::tc_fence_after();
@@ -517,11 +550,11 @@ static int make_map(CUtensorMap* m, const void* base, int64_t rows, int64_t K, i
                ? MXQ_OK : MXQ_ERR_CUDA;
 }
 
-template <int NT>
-static int launch_fp8(const CUtensorMap& tp, const CUtensorMap& tq, const Fp8Gemm& g, cudaStream_t st) {
-    using S = Fp8Tile<NT>;
-    static_assert(S::kTotal <= 232448, "shared memory");
-    auto kern = fp8_gemm_kernel<NT>;
+template <int NT, bool SPLIT>
+static int launch_fp8_split(const CUtensorMap& tp, const CUtensorMap& tq, const Fp8Gemm& g, cudaStream_t st) {
+    using S = Fp8Tile<NT, SPLIT>;
+    static_assert(S::kTotal <= (NT == 128 ? 232448 : 115712), "shared memory of one CTA an SM, or of two");
+    auto kern = fp8_gemm_kernel<NT, SPLIT>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kTotal) != cudaSuccess) { cudaGetLastError(); return MXQ_ERR_CUDA; }
     const int64_t grid = g.p_tiles * g.q_tiles * g.split;
     if (grid > 0x7fffffff) return MXQ_ERR_TOO_LARGE;
@@ -530,13 +563,20 @@ static int launch_fp8(const CUtensorMap& tp, const CUtensorMap& tq, const Fp8Gem
     cfg.blockDim = dim3(S::kThreads);
     cfg.dynamicSmemBytes = S::kTotal;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = g.split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = g.early ? 2 : 1;
     if (cudaLaunchKernelEx(&cfg, kern, tp, tq, g) != cudaSuccess) { cudaGetLastError(); return MXQ_ERR_CUDA; }
     return check_launch();
+}
+
+template <int NT>
+static int launch_fp8(const CUtensorMap& tp, const CUtensorMap& tq, const Fp8Gemm& g, cudaStream_t st) {
+    return g.split > 1 ? launch_fp8_split<NT, true>(tp, tq, g, st) : launch_fp8_split<NT, false>(tp, tq, g, st);
 }
 
 // out [M, N]: boxes of 32 rows x 128 bytes
@@ -583,29 +623,73 @@ int fp8_gemm_status(int clear) {
 
 }  // namespace mxq
 
-extern "C" int mxq_fp8_gemm(const void* a, int64_t a_pitch, const float* a_scales, int a_tile, int a_fmt, const void* b,
-                            int64_t b_pitch, const float* b_scales, int b_tile, int b_fmt, void* out, int out_dtype,
-                            const void* bias, int bias_dtype, int64_t M, int64_t N, int64_t K, void* stream) {
-    using namespace mxq;
+namespace mxq {
+// Which kernel and shape.  A kernel's time is the number of rounds its CTAs need on the GPU times what one CTA takes, a fixed part
+// (launch, barriers, tensor memory, first loads, join and store: about 4.5 us) and a part for each K block it walks.  The
+// latter, measured: 0.30, 0.36, 0.41 and 0.66 us with 16, 32, 64 and 128 rows of a to a tile (the first bound by a CTA's
+// own loads, the last by the scaling of the sums), or what HBM needs for the 16 KB of b that every CTA at work reads;
+// 0.60 us for a CTA pair on 256 x 256, 1.1 us where b has a scale a row.  Both sides of each border (us):
+// 64 x 4096 x 4096 split 1 / 2 / 4 / 8: 16.8 / 12.1 / 9.4 / 19.0; 1 x 8192 x 8192 (weights from HBM): 28.1 / 20.2 / 18.3 / 20.5,
+// 1 x 28672 x 8192: 42.9 / 49.8 / 56.0 / 61.5; 128 x 4096 x 4096
+// with 64 rows, split 2: 12.6, with 128 rows, split 4: 12.9; 1024 x 1024 x 1024 64 rows 8.2, 128 rows 11.3;
+// 2048 x 2048 x 2048 pair 14.3, 128 rows 31.0.
+struct Fp8Plan { int nt, split; };                 // nt 0: CTA pairs
+static Fp8Plan plan_fp8(int64_t M, int64_t N, int64_t blocks, bool b_rows, bool tma_out) {
+    const double sms = sm_count(), fixed = 4.5, hbm = 5.5e6;       // us, bytes a us
+    const double block_us[4] = {0.30, 0.36, 0.41, 0.66};
+    Fp8Plan best = {16, 1};
+    double best_us = 1e300;
+    for (int i = 0; i < 4; ++i) {
+        const int nt = 16 << i;
+        if (i > 0 && M <= nt / 2) break;           // half of the tile would be empty
+        if (M > nt && nt < 64) continue;           // b would be read for several tiles of few rows
+        const double p_tiles = (double)((N + 127) / 128), tiles = p_tiles * (double)((M + nt - 1) / nt);
+        for (int split = 1; split <= 8; split *= 2) {
+            if (split > 1 && blocks < 2 * split) break;
+            // two CTAs on an SM below 128 rows; clusters of four and more leave some SMs of a GPC idle
+            const double slots = sms * (nt < 128 ? 2 : 1) * (split >= 4 ? 0.875 : 1);
+            const double rounds = ceil(tiles * split / slots), busy = tiles * split / rounds;
+            const double share = nt < 128 && busy > sms ? 2 : 1;   // two CTAs on an SM share its tensor core and its fp32 pipes
+            const double per = fmax(block_us[i] * (nt > 32 ? share : 1), fmin(busy, p_tiles * split / rounds) * 16384 / hbm);
+            const double us = rounds * (fixed + (double)((blocks + split - 1) / split) * per);
+            if (us < best_us) { best_us = us; best = {nt, split}; }
+        }
+    }
+    if (M > 128 && N > 128) {
+        const double rounds = ceil((double)((M + 255) / 256) * (double)((N + 255) / 256) / (sms / 2));
+        // rows of no multiple of 16 bytes leave by single stores, 8 us a tile
+        if (fixed + rounds * ((double)blocks * (b_rows ? 1.1 : 0.60) + (tma_out ? 0 : 8)) < best_us) best = {0, 1};
+    }
+    return best;
+}
+
+// `early`: b was complete before the kernel in front of this launch began
+int fp8_gemm(const void* a, int64_t a_pitch, const float* a_scales, int a_tile, int a_fmt, const void* b, int64_t b_pitch,
+             const float* b_scales, int b_tile, int b_fmt, void* out, int out_dtype, const void* bias, int bias_dtype, int64_t M,
+             int64_t N, int64_t K, bool early, cudaStream_t st) {
     if (M < 0 || N < 0 || K <= 0 || a_fmt < 0 || a_fmt > 1 || b_fmt < 0 || b_fmt > 1) return MXQ_ERR_BAD_ARG;
     if (out_dtype < 0 || out_dtype > 2 || (bias && (bias_dtype < 0 || bias_dtype > 2))) return MXQ_ERR_BAD_ARG;
     if (M == 0 || N == 0) return MXQ_OK;
     if (!a || !b || !a_scales || !b_scales || !out || a_pitch < K || b_pitch < K) return MXQ_ERR_BAD_ARG;
-    if (!aligned16(a) || !aligned16(b) || a_pitch % 16 || b_pitch % 16) return MXQ_ERR_ALIGN;
+    if (!aligned16(a) || !aligned16(b) || !aligned16(out) || a_pitch % 16 || b_pitch % 16) return MXQ_ERR_ALIGN;
+    // coordinates are 32-bit, and a block or eight times a block count is added to them
     if (M > 0x7fffff00 || N > 0x7fffff00 || K > 0x7fffff00) return MXQ_ERR_TOO_LARGE;
-    cudaStream_t st = (cudaStream_t)stream;
-    const int64_t tiles2 = ((M + 255) / 256) * ((N + 255) / 256);
-    if (M >= 256 && N >= 256 && tiles2 >= sm_count() / 4) {                                // pairs of CTAs where at least half of the pairs have a tile
+    const int64_t blocks = (K + 127) / 128;
+    const bool tma_out = (N * dtype_size(out_dtype)) % 16 == 0;
+    const Fp8Plan plan = plan_fp8(M, N, blocks, !b_tile, tma_out);
+    CUtensorMap ta, tb, tc;
+    int rc;
+    if (plan.nt == 0) {
         Fp8Pair g;
         g.sa = a_scales; g.sa_shift = a_tile ? 7 : 0; g.sa_ld = a_tile ? (M + 127) / 128 : M;
         g.sb = b_scales; g.sb_shift = b_tile ? 7 : 0; g.sb_ld = b_tile ? (N + 127) / 128 : N;
         g.out = out; g.out_dtype = out_dtype; g.bias = bias; g.bias_dtype = bias_dtype;
-        g.M = M; g.N = N; g.kb_total = (K + 127) / 128;
+        g.M = M; g.N = N; g.kb_total = blocks;
         g.m_tiles = (M + 255) / 256; g.n_tiles = (N + 255) / 256;
         g.idesc = ptx::idesc_f8(a_fmt, b_fmt, 256, 256);
-        g.tma_out = aligned16(out) && (N * dtype_size(out_dtype)) % 16 == 0;
-        CUtensorMap ta, tb, tc;
-        int rc = make_map(&ta, a, M, K, a_pitch, 128);
+        g.tma_out = tma_out;
+        if (g.m_tiles * g.n_tiles + sm_count() > 0x7fffffff) return MXQ_ERR_TOO_LARGE;
+        rc = make_map(&ta, a, M, K, a_pitch, 128);
         if (!rc) rc = make_map(&tb, b, N, K, b_pitch, 128);
         tc = ta;
         if (!rc && g.tma_out) rc = make_out_map(&tc, out, M, N, out_dtype);
@@ -614,26 +698,32 @@ extern "C" int mxq_fp8_gemm(const void* a, int64_t a_pitch, const float* a_scale
         if (out_dtype == MXQ_F32) return g.sb_shift ? launch_fp8_pair<false, true>(ta, tb, tc, g, st) : launch_fp8_pair<true, true>(ta, tb, tc, g, st);
         return g.sb_shift ? launch_fp8_pair<false, false>(ta, tb, tc, g, st) : launch_fp8_pair<true, false>(ta, tb, tc, g, st);
     }
-    const int nt = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+    const int nt = plan.nt;
     Fp8Gemm g;
     g.sp = b_scales; g.sp_shift = b_tile ? 7 : 0; g.sp_ld = b_tile ? (N + 127) / 128 : N;
     g.sq = a_scales; g.sq_shift = a_tile ? 7 : 0; g.sq_ld = a_tile ? (M + 127) / 128 : M;
     g.out = out; g.out_dtype = out_dtype; g.bias = bias; g.bias_dtype = bias_dtype;
-    g.P = N; g.Q = M; g.kb_total = (K + 127) / 128;
+    g.P = N; g.Q = M; g.kb_total = blocks;
     g.p_tiles = (N + 127) / 128; g.q_tiles = (M + nt - 1) / nt;
     g.idesc = ptx::idesc_f8(b_fmt, a_fmt, 128, nt);
-    // K blocks are split until every SM has a CTA, as long as each CTA keeps two of them
-    g.split = 1;
-    while (g.split < 8 && g.p_tiles * g.q_tiles * g.split < sm_count() && g.kb_total >= 4 * g.split) g.split *= 2;
-    CUtensorMap tp, tq;
-    int rc = make_map(&tp, b, N, K, b_pitch, 128);
-    if (!rc) rc = make_map(&tq, a, M, K, a_pitch, nt);
+    g.split = plan.split;
+    g.early = early;
+    rc = make_map(&tb, b, N, K, b_pitch, 128);
+    if (!rc) rc = make_map(&ta, a, M, K, a_pitch, nt);
     if (rc) return rc;
     g_launch_count[0].fetch_add(1, std::memory_order_relaxed);
-    if (nt == 16) return launch_fp8<16>(tp, tq, g, st);
-    if (nt == 32) return launch_fp8<32>(tp, tq, g, st);
-    if (nt == 64) return launch_fp8<64>(tp, tq, g, st);
-    return launch_fp8<128>(tp, tq, g, st);
+    if (nt == 16) return launch_fp8<16>(tb, ta, g, st);
+    if (nt == 32) return launch_fp8<32>(tb, ta, g, st);
+    if (nt == 64) return launch_fp8<64>(tb, ta, g, st);
+    return launch_fp8<128>(tb, ta, g, st);
+}
+}  // namespace mxq
+
+extern "C" int mxq_fp8_gemm(const void* a, int64_t a_pitch, const float* a_scales, int a_tile, int a_fmt, const void* b,
+                            int64_t b_pitch, const float* b_scales, int b_tile, int b_fmt, void* out, int out_dtype,
+                            const void* bias, int bias_dtype, int64_t M, int64_t N, int64_t K, void* stream) {
+    return mxq::fp8_gemm(a, a_pitch, a_scales, a_tile, a_fmt, b, b_pitch, b_scales, b_tile, b_fmt, out, out_dtype, bias, bias_dtype,
+                         M, N, K, false, (cudaStream_t)stream);
 }
 
 extern "C" int64_t mxq_fp8_linear_workspace_bytes(int64_t M, int64_t K) {
@@ -654,8 +744,9 @@ extern "C" int mxq_fp8_linear_fwd(const void* x, int x_dtype, int64_t x_stride, 
     float* scales = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (M * pitch + 255) / 256 * 256);
     const int rc = mxq_fp8_quantize(x, x_dtype, M, K, x_stride, x_fmt, 0, workspace, pitch, scales, nullptr, 0, nullptr, nullptr, stream);
     if (rc) return rc;
-    return mxq_fp8_gemm(workspace, pitch, scales, 0, x_fmt, w, w_pitch, w_scales, w_tile, w_fmt, y, y_dtype, bias, bias_dtype,
-                        M, N, K, stream);
+    // the product may load weights while x is still being quantized: only that kernel lies between them and their last writer
+    return mxq::fp8_gemm(workspace, pitch, scales, 0, x_fmt, w, w_pitch, w_scales, w_tile, w_fmt, y, y_dtype, bias, bias_dtype,
+                         M, N, K, true, (cudaStream_t)stream);
 }
 
 // ---------------------------------------------------------------------------------------------------------------

@@ -13,6 +13,7 @@
 // as whole 128-byte rows of the transposed operand.
 #include "mxq_common.cuh"
 #include "fp8_block.cuh"
+#include "sm100_ptx.cuh"
 
 namespace mxq {
 
@@ -83,6 +84,7 @@ fp8_quantize_kernel(const QuantArgs g, const bool tile) {
     __shared__ float warp_part[8];
     __shared__ float col_r[128];
     __shared__ uint2 stage[128][16];
+    ptx::grid_launch_dependents();               // a product launched to overlap waits for this grid before it reads its results
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int l16 = lane & 15, h = lane >> 4;
     const int64_t cb = blockIdx.x % g.col_blocks, rb = blockIdx.x / g.col_blocks;
