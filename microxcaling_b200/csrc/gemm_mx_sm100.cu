@@ -848,6 +848,6 @@ extern "C" int mxq_device_status(int clear) {
     int v = 0;
     if (cudaMemcpy(&v, w, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return MXQ_ERR_CUDA;
     if (clear && v != 0) cudaMemset(w, 0, sizeof(int));
-    const int f = mxq::fp8_gemm_status(clear);
-    return v != 0 ? v : f;
+    const int f = mxq::fp8_gemm_status(clear), n = mxq::norm_status(clear);
+    return v != 0 ? v : f != 0 ? f : n;
 }
