@@ -476,17 +476,17 @@ int mxq_layer_norm_bwd(const void* dy, const void* x, int dtype, int64_t dy_stri
  * Log probabilities of given tokens under softmax(logits * inv_temperature), entropies and the best alternatives.
  *   logits     [rows, vocab] of dtype, stride elements from row to row
  *   tokens     [rows] or NULL; ignore_index gives 0, any other index outside [0, vocab) gives NaN
- *   logprobs   [rows] fp32 (with tokens); entropy, lse: [rows] fp32 or NULL (lse is what the gradient needs)
+ *   logprobs   [rows] fp32 (with tokens); entropy [rows] fp32 or NULL; stats [rows, 2] fp32 or NULL: what the gradient needs
  *   top        0 .. 32: the largest logits, largest first, the lowest index first among equals (NaN above all):
  *              their log probabilities [rows, top] fp32 and indices [rows, top]
  * A row with no logit above -inf has log probability -inf, entropy 0 and gradient 0.
  * Gradient of sum(g_logprobs * logprobs) + sum(g_entropy * entropy): grad [rows, vocab] of dtype; either g may be NULL.
  */
 int mxq_token_logprobs(const void* logits, int dtype, int64_t stride, const int64_t* tokens, int64_t ignore_index,
-                       float inv_temperature, float* logprobs, float* entropy, float* lse, int top, float* top_logprobs,
+                       float inv_temperature, float* logprobs, float* entropy, float* stats, int top, float* top_logprobs,
                        int64_t* top_tokens, int64_t rows, int64_t vocab, void* stream);
 int mxq_token_logprobs_grad(const void* logits, int dtype, int64_t stride, const int64_t* tokens, int64_t ignore_index,
-                            float inv_temperature, const float* lse, const float* entropy, const float* g_logprobs,
+                            float inv_temperature, const float* stats, const float* entropy, const float* g_logprobs,
                             const float* g_entropy, void* grad, int64_t rows, int64_t vocab, void* stream);
 
 /* Reads (and optionally clears) the current device's status words: 0, or

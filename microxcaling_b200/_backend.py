@@ -712,27 +712,27 @@ def layer_norm_bwd(dy, x, weight, mean, rstd, sums_dtype, need):
 LOGPROBS_MAX_TOP = 32
 
 
-def token_logprobs(x, tokens, ignore_index, inv_t, entropy, top, want_lse):
-    """(logprobs, entropy, lse, top logprobs, top tokens) of x [rows, vocab]; None for what is not wanted; see mxq_token_logprobs."""
+def token_logprobs(x, tokens, ignore_index, inv_t, entropy, top, want_stats):
+    """(logprobs, entropy, statistics for the gradient, top logprobs, top tokens) of x [rows, vocab]; None for what is not wanted; see mxq_token_logprobs."""
     rows, vocab = x.shape
     lp = x.new_empty(rows, dtype=torch.float32) if tokens is not None else None
     h = x.new_empty(rows, dtype=torch.float32) if entropy else None
-    lse = x.new_empty(rows, dtype=torch.float32) if want_lse else None
+    stats = x.new_empty((rows, 2), dtype=torch.float32) if want_stats else None
     tlp = x.new_empty((rows, top), dtype=torch.float32) if top else None
     tok = x.new_empty((rows, top), dtype=torch.int64) if top else None
     with _device_of(x.device):
         check(lib().mxq_token_logprobs(_ptr(x), _DT[x.dtype], x.stride(0) if rows > 1 else vocab, _ptr(tokens), ignore_index, inv_t,
-                                       _ptr(lp), _ptr(h), _ptr(lse), top, _ptr(tlp), _ptr(tok), rows, vocab, _stream(x)))
-    return lp, h, lse, tlp, tok
+                                       _ptr(lp), _ptr(h), _ptr(stats), top, _ptr(tlp), _ptr(tok), rows, vocab, _stream(x)))
+    return lp, h, stats, tlp, tok
 
 
-def token_logprobs_grad(x, tokens, ignore_index, inv_t, lse, entropy, g_lp, g_h):
+def token_logprobs_grad(x, tokens, ignore_index, inv_t, stats, entropy, g_lp, g_h):
     """Gradient [rows, vocab] with respect to x; see mxq_token_logprobs_grad."""
     rows, vocab = x.shape
     dx = x.new_empty((rows, vocab))
     with _device_of(x.device):
         check(lib().mxq_token_logprobs_grad(_ptr(x), _DT[x.dtype], x.stride(0) if rows > 1 else vocab, _ptr(tokens), ignore_index,
-                                            inv_t, _ptr(lse), _ptr(entropy), _ptr(g_lp), _ptr(g_h), _ptr(dx), rows, vocab,
+                                            inv_t, _ptr(stats), _ptr(entropy), _ptr(g_lp), _ptr(g_h), _ptr(dx), rows, vocab,
                                             _stream(x)))
     return dx
 

@@ -15,22 +15,22 @@ _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 TokenLogprobs = collections.namedtuple("TokenLogprobs", "logprobs entropy top_logprobs top_tokens")
 
 
-def _run(x, tokens, top, entropy, inv_t, ignore_index, want_lse):
-    """(rows of x, tokens, log sum, entropy as the kernel wrote them; the outputs in the shape of x's leading dimensions)"""
+def _run(x, tokens, top, entropy, inv_t, ignore_index, want_stats):
+    """(rows of x, tokens, statistics, entropy as the kernel wrote them; the outputs in the shape of x's leading dimensions)"""
     x2 = _backend.rows_of(x)
     t = None if tokens is None else tokens.reshape(-1).contiguous()
-    lp, h, lse, tlp, tok = _backend.token_logprobs(x2, t, ignore_index, inv_t, entropy, top, want_lse)
+    lp, h, stats, tlp, tok = _backend.token_logprobs(x2, t, ignore_index, inv_t, entropy, top, want_stats)
     out = (lp, h, tlp, tok)
     if x.dim() != 2:
         out = tuple(None if o is None else o.view(x.shape[:-1] + o.shape[1:]) for o in out)
-    return x2, t, lse, h, out
+    return x2, t, stats, h, out
 
 
 class TokenLogprobsFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, tokens, top, entropy, inv_t, ignore_index):
-        x2, t, lse, h, out = _run(x, tokens, top, entropy, inv_t, ignore_index, True)
-        ctx.save_for_backward(x2, t, lse, h)
+        x2, t, stats, h, out = _run(x, tokens, top, entropy, inv_t, ignore_index, True)
+        ctx.save_for_backward(x2, t, stats, h)
         ctx.args = (inv_t, ignore_index, x.shape)
         ctx.set_materialize_grads(False)
         if top:
@@ -40,12 +40,12 @@ class TokenLogprobsFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g_lp, g_h, g_tlp, g_tok):
-        x2, t, lse, h = ctx.saved_tensors
+        x2, t, stats, h = ctx.saved_tensors
         inv_t, ignore_index, shape = ctx.args
         if g_lp is None and g_h is None:
             return (None,) * 6
         flat = [None if g is None else g.reshape(-1).contiguous() for g in (g_lp, g_h)]
-        dx = _backend.token_logprobs_grad(x2, t, ignore_index, inv_t, lse, h, *flat)
+        dx = _backend.token_logprobs_grad(x2, t, ignore_index, inv_t, stats, h, *flat)
         return dx.view(shape), None, None, None, None, None
 
 
