@@ -280,11 +280,16 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
 // ---------------------------------------------------------------------------------------------------------------
 // Large products: CTA pairs (cta_group::2) on 256 x 256 tiles, persistent.  The tensor core's rows are a's here.  Each CTA
 // stages its own 128 rows of a and its half of b's 256 rows (32 KB a K block, five of them in flight), the even CTA issues the
-// MMAs for both, and every CTA's eight epilogue warps hold 128 x 256 fp32 sums in registers, 128 columns of a row a thread.
+// MMAs for both, and every CTA's eight epilogue warps hold 128 x 256 fp32 sums in registers, 128 a thread.
 // The two accumulators of 256 columns fill tensor memory: while the warps scale and add one block's sums the tensor core
-// works on the next one.  What has to fit beside its 512 cycles a block (128 x 256 x 128 at the peak rate on each SM) is
-// 32768 fused multiply-adds, 256 cycles of the fp32 pipes, and the 64 cycles in which the block leaves tensor memory;
-// with a scale for every row of b as well (B_ROWS: weight gradients) there is a second multiplication, and the fp32 pipes become the limit.
+// works on the next one.  Beside its 512 cycles a block (128 x 256 x 128 at the peak rate on each SM) stand 32768 fused
+// multiply-adds, 256 cycles of the fp32 pipes (twice that with a scale for every row of b as well, B_ROWS: weight gradients).
+//
+// Measured: 8192 x 4096 x 4096 135 to 145 us (1.9 to 2.0 PFLOP/s), 16384 x 28672 x 8192 3.4 ms (2.25 PFLOP/s, SM clock near
+// 1.4 GHz under the power cap); with B_ROWS 4096 x 4096 x 8192 259 us (1.06 PFLOP/s; 281 us when every thread held one row and
+// read all column scales).  With the scaling left out the same loop takes 119 us and 2.7 ms: the rest is the hand-over of the accumulators
+// (two of them, a round trip of a block's MMAs, drain and arrival each), not the arithmetic.  Tried and dropped: a release
+// fence at that hand-over (299 instead of 181 us at that stage), halves of an accumulator handed over apart (194 to 177).
 // ---------------------------------------------------------------------------------------------------------------
 struct Fp8Pair {
     const float* sa;
@@ -411,72 +416,97 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
         uint32_t ring = 0;
         uint32_t it = 0;
         bool ok = true;
+        // Which sums a thread holds, as 64 pairs of neighbouring columns.  With one scale of b for the tile's 128 columns: all of one
+        // row.  With a scale a column: four rows (lane / 4 + 8 k) and every fourth pair of columns, so that a thread needs 32 of
+        // the 128 column scales and not all of them (128 floats to each of 256 threads a block are 1024 cycles of shared memory).
+        constexpr int R = B_ROWS ? 4 : 1;
+        auto row_of = [&](int k) { return B_ROWS ? (lane >> 2) + 8 * k : lane; };
         // the scales of the next block are fetched a block ahead
         int64_t mt = 0, nt = 0;
-        float sa_next = 0.f, sb_next = 0.f;
+        float sa_next[R], sb_next = 0.f;
         const float *sap = nullptr, *sbp = nullptr;
+        int sa_row = 0;
+        auto fetch_a = [&]() {
+#pragma unroll
+            for (int k = 0; k < R; ++k) sa_next[k] = __ldg(sap + (min(sa_row + 8 * k, (int)g.M - 1) >> g.sa_shift));
+        };
         auto aim = [&](int64_t t) {
             pair_tile(t, g, mt, nt);
-            const int64_t row = mt * 256 + rank * 128 + quarter * 32 + lane;
-            sap = g.sa + (min(row, g.M - 1) >> g.sa_shift);
+            sa_row = (int)(mt * 256 + rank * 128 + quarter * 32) + row_of(0);
+            sap = g.sa;
+            fetch_a();
             const int64_t col = nt * 256 + half * 128 + (B_ROWS ? te : 0);
-            sbp = g.sb + (min(col, g.N - 1) >> g.sb_shift);
-            sa_next = __ldg(sap);
-            sb_next = __ldg(sbp);
+            sb_next = __ldg(sbp = g.sb + (min(col, g.N - 1) >> g.sb_shift));
         };
         if (pair < total) aim(pair);
         for (int64_t t = pair; t < total && ok; t += pairs) {
             const int64_t row0 = mt * 256 + rank * 128 + quarter * 32, col0 = nt * 256 + half * 128;
-            float2 acc[64];                                  // pairs of columns
+            float2 acc[64];
 #pragma unroll
             for (int i = 0; i < 64; ++i) acc[i] = make_float2(0.f, 0.f);
             for (int64_t kb = 0; kb < g.kb_total; ++kb, ++it) {
                 const uint32_t b = it & 1;
-                const float sa = sa_next;
-                const uint64_t f = B_ROWS ? ptx::pack2f(sa, sa) : ptx::pack2f(sa * sb_next, sa * sb_next);
-                const float* bs = b_scale + b * 256 + half * 128;
+                uint64_t f[R];
+#pragma unroll
+                for (int k = 0; k < R; ++k) {
+                    const float v = B_ROWS ? sa_next[k] : sa_next[k] * sb_next;
+                    f[k] = ptx::pack2f(v, v);
+                }
+                const float* bs = b_scale + b * 256 + half * 128 + 2 * (lane & 3);
                 if constexpr (B_ROWS) b_scale[b * 256 + half * 128 + te] = sb_next;
                 if (kb + 1 < g.kb_total) {
-                    sa_next = __ldg(sap += g.sa_ld);
+                    sap += g.sa_ld;
+                    fetch_a();
                     sb_next = __ldg(sbp += g.sb_ld);
                 }
                 if constexpr (B_ROWS) asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");   // two buffers: a warp is at most one block ahead
-                if (!ptx::mbar_wait(ptx::smem_u32(&acc_full[b]), (it >> 1) & 1, abort_flag)) {
+                if (!ptx::mbar_wait(ptx::smem_u32(&acc_full[b]), (it >> 1) & 1, abort_flag))
                     ok = false;                                // counts the blocks to the end all the same: every later wait gives up at once
-                }
                 ptx::tc_fence_after();
                 const uint32_t ta = tmem_base + ((uint32_t)(quarter * 32) << 16) + b * 256 + half * 128;
+                auto drained = [&]() {                         // the accumulator is out of tensor memory
+                    ptx::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive_cluster_tmem(ptx::mapa(ptx::smem_u32(&acc_empty[b]), 0));
+                };
+                if constexpr (B_ROWS) {
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t w[64];
-                    ptx::tmem_ld_32x32b_x32(ta + 64 * c, w);
-                    ptx::tmem_ld_32x32b_x32(ta + 64 * c + 32, w + 32);
-                    ptx::tmem_ld_wait();
-                    if (c == 1) {                              // the accumulator is out of tensor memory
-                        ptx::tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) ptx::mbar_arrive_cluster_tmem(ptx::mapa(ptx::smem_u32(&acc_empty[b]), 0));
-                    }
+                    for (int c = 0; c < 4; ++c) {              // 64 columns of 16 rows: this thread's pairs in two rows
+                        uint32_t w[32];
+                        ptx::tmem_ld_16x256b_x8(ta + 64 * (c >> 1) + ((c & 1) * 16u << 16), w);
+                        ptx::tmem_ld_wait();
+                        if (c == 3) drained();
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        uint64_t m0 = f, m1 = f;
-                        if constexpr (B_ROWS) {
-                            const float4 q = *reinterpret_cast<const float4*>(bs + 64 * c + 2 * i);
-                            m0 = ptx::mul2(f, ptx::pack2f(q.x, q.y));
-                            m1 = ptx::mul2(f, ptx::pack2f(q.z, q.w));
+                        for (int n = 0; n < 8; ++n) {
+                            const uint64_t q = *reinterpret_cast<const uint64_t*>(bs + 64 * (c >> 1) + 8 * n);
+#pragma unroll
+                            for (int k = 0; k < 2; ++k)
+                                scale_add(acc[32 * (c >> 1) + 8 * (2 * (c & 1) + k) + n], w[4 * n + 2 * k], w[4 * n + 2 * k + 1],
+                                          ptx::mul2(f[2 * (c & 1) + k], q));
                         }
-                        scale_add(acc[32 * c + i], w[2 * i], w[2 * i + 1], m0);
-                        scale_add(acc[32 * c + i + 1], w[2 * i + 2], w[2 * i + 3], m1);
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t w[64];
+                        ptx::tmem_ld_32x32b_x32(ta + 64 * c, w);
+                        ptx::tmem_ld_32x32b_x32(ta + 64 * c + 32, w + 32);
+                        ptx::tmem_ld_wait();
+                        if (c == 1) drained();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) scale_add(acc[32 * c + i], w[2 * i], w[2 * i + 1], f[0]);
                     }
                 }
             }
             if (t + pairs < total) aim(t + pairs);
             if (!ok || row0 >= g.M || col0 >= g.N) continue;
+            // first column of pair i
+            auto column = [&](int i) { return B_ROWS ? 64 * (i >> 5) + 8 * (i & 7) + 2 * (lane & 3) : 2 * i; };
             if (g.bias) {
 #pragma unroll
                 for (int i = 0; i < 64; ++i) {
-                    acc[i].x += load_dyn(g.bias, g.bias_dtype, min(col0 + 2 * i, g.N - 1));
-                    acc[i].y += load_dyn(g.bias, g.bias_dtype, min(col0 + 2 * i + 1, g.N - 1));
+                    acc[i].x += load_dyn(g.bias, g.bias_dtype, min(col0 + column(i), g.N - 1));
+                    acc[i].y += load_dyn(g.bias, g.bias_dtype, min(col0 + column(i) + 1, g.N - 1));
                 }
             }
             // out through boxes of 32 rows x 128 bytes in the 128-byte swizzle of the output's tensor map
@@ -486,27 +516,43 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
                 const int64_t col = col0 + PER * c;
                 if (col >= g.N) break;
                 uint8_t* box = smem + boxes + (ring++ % S::kBoxes) * 4096;
+                const uint32_t box_s = ptx::smem_u32(box);
                 if (lane == 0) ptx::bulk_wait_read<S::kBoxes - 1>();       // this box's last store has read it
                 __syncwarp();
+                if constexpr (B_ROWS) {
 #pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    uint32_t w[4];
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t at = box_s + row_of(k) * 128;       // row % 8 = lane / 4
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if constexpr (F32) {
-                            const float2 p = acc[16 * c + 2 * q + (j >> 1)];
-                            w[j] = __float_as_uint(j & 1 ? p.y : p.x);
-                        } else {
-                            const float2 p = acc[32 * c + 4 * q + j];
-                            w[j] = pack2(p.x, p.y, g.out_dtype);
+                        for (int n = 0; n < PER / 8; ++n) {
+                            const float2 p = F32 ? acc[32 * (c >> 1) + 8 * k + 4 * (c & 1) + n] : acc[32 * c + 8 * k + n];
+                            if constexpr (F32)
+                                ptx::st_shared_v2(at + (((2 * n + ((lane & 3) >> 1)) ^ (lane >> 2)) << 4) + 8 * (lane & 1), __float_as_uint(p.x), __float_as_uint(p.y));
+                            else
+                                ptx::st_shared(at + ((n ^ (lane >> 2)) << 4) + 4 * (lane & 3), pack2(p.x, p.y, g.out_dtype));
                         }
                     }
-                    ptx::st_shared_v4(ptx::smem_u32(box) + lane * 128 + ((q ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if constexpr (F32) {
+                                const float2 p = acc[16 * c + 2 * q + (j >> 1)];
+                                w[j] = __float_as_uint(j & 1 ? p.y : p.x);
+                            } else {
+                                const float2 p = acc[32 * c + 4 * q + j];
+                                w[j] = pack2(p.x, p.y, g.out_dtype);
+                            }
+                        }
+                        ptx::st_shared_v4(box_s + lane * 128 + ((q ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
+                    }
                 }
                 if (g.tma_out) {
                     ptx::fence_proxy_async();
                     __syncwarp();
-                    if (lane == 0) { ptx::tma_store_2d(&tmap_c, ptx::smem_u32(box), (int)col, (int)row0); ptx::bulk_commit(); }
+                    if (lane == 0) { ptx::tma_store_2d(&tmap_c, box_s, (int)col, (int)row0); ptx::bulk_commit(); }
                 } else {                                       // rows that are no multiple of 16 bytes long
                     __syncwarp();
                     const int n = (int)min((int64_t)32, g.M - row0);
@@ -628,7 +674,7 @@ namespace mxq {
 // (launch, barriers, tensor memory, first loads, join and store: about 4.5 us) and a part for each K block it walks.  The
 // latter, measured: 0.30, 0.36, 0.41 and 0.66 us with 16, 32, 64 and 128 rows of a to a tile (the first bound by a CTA's
 // own loads, the last by the scaling of the sums), or what HBM needs for the 16 KB of b that every CTA at work reads;
-// 0.60 us for a CTA pair on 256 x 256, 1.1 us where b has a scale a row.  Both sides of each border (us):
+// 0.60 us for a CTA pair on 256 x 256, 1.0 us where b has a scale a row.  Both sides of each border (us):
 // 64 x 4096 x 4096 split 1 / 2 / 4 / 8: 16.8 / 12.1 / 9.4 / 19.0; 1 x 8192 x 8192 (weights from HBM): 28.1 / 20.2 / 18.3 / 20.5,
 // 1 x 28672 x 8192: 42.9 / 49.8 / 56.0 / 61.5; 128 x 4096 x 4096
 // with 64 rows, split 2: 12.6, with 128 rows, split 4: 12.9; 1024 x 1024 x 1024 64 rows 8.2, 128 rows 11.3;
@@ -658,7 +704,7 @@ static Fp8Plan plan_fp8(int64_t M, int64_t N, int64_t blocks, bool b_rows, bool 
     if (M > 128 && N > 128) {
         const double rounds = ceil((double)((M + 255) / 256) * (double)((N + 255) / 256) / (sms / 2));
         // rows of no multiple of 16 bytes leave by single stores, 8 us a tile
-        if (fixed + rounds * ((double)blocks * (b_rows ? 1.1 : 0.60) + (tma_out ? 0 : 8)) < best_us) best = {0, 1};
+        if (fixed + rounds * ((double)blocks * (b_rows ? 1.0 : 0.60) + (tma_out ? 0 : 8)) < best_us) best = {0, 1};
     }
     return best;
 }
