@@ -38,6 +38,13 @@ struct Fp8Gemm {
     uint32_t idesc;
 };
 
+// After a wait that gave up: the status word, and a millisecond in which copies still in flight land before the CTA leaves.
+__device__ __forceinline__ void give_up(int aborted) {
+    if (!aborted) return;
+    atomicExch(&g_fp8_status, MXQ_ERR_DEVICE);
+    for (int i = 0; i < 64; ++i) __nanosleep(16384);
+}
+
 __device__ __forceinline__ float load_dyn(const void* p, int dtype, int64_t i) {
     if (dtype == DT_F32) return load1<DT_F32>(p, i);
     if (dtype == DT_F16) return load1<DT_F16>(p, i);
@@ -153,16 +160,11 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
 
     if (warp == 0) {
         if (producer) {
-            bool ok = true;
             for (int i = S::kStages; i < n_kb; ++i) {
-                if (!ptx::mbar_wait(ptx::smem_u32(&empty[i % S::kStages]), ((i / S::kStages) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                if (!ptx::mbar_wait(ptx::smem_u32(&empty[i % S::kStages]), ((i / S::kStages) & 1) ^ 1, abort_flag)) break;
                 load_p(i);
                 load_q(i);
             }
-            if (!ok)                               // give copies already in flight a bounded time to land
-                for (int s = 0; s < S::kStages; ++s)
-                    for (uint32_t i = 0; i < 4096 && !ptx::mbar_try_wait(ptx::smem_u32(&full[s]), 0) &&
-                                         !ptx::mbar_try_wait(ptx::smem_u32(&full[s]), 1); ++i) __nanosleep(64);
         }
         __syncwarp();
         if constexpr (SPLIT) ptx::cluster_wait();
@@ -270,7 +272,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
     }
     ptx::tc_fence_before();
     __syncthreads();
-    if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_fp8_status, MXQ_ERR_DEVICE);
+    if (threadIdx.x == 0) give_up(*abort_flag);
     if (warp == 1) {
         ptx::tc_fence_after();
         ptx::tmem_dealloc(tmem_base, S::kTmemCols);
@@ -574,9 +576,10 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     }
     ptx::tc_fence_before();
     __syncthreads();
+    if (threadIdx.x == 0) give_up(*abort_flag);
+    __syncwarp();
     ptx::cluster_arrive();                                    // the partner no longer touches this CTA's memory
     ptx::cluster_wait();
-    if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_fp8_status, MXQ_ERR_DEVICE);
     if (warp == 1) {
         ptx::tc_fence_after();
         ptx::tmem_dealloc_pair(tmem_base, 512);
@@ -672,8 +675,8 @@ int fp8_gemm_status(int clear) {
 namespace mxq {
 // Which kernel and shape.  A kernel's time is the number of rounds its CTAs need on the GPU times what one CTA takes, a fixed part
 // (launch, barriers, tensor memory, first loads, join and store: about 4.5 us) and a part for each K block it walks.  The
-// latter, measured: 0.30, 0.36, 0.41 and 0.66 us with 16, 32, 64 and 128 rows of a to a tile (the first bound by a CTA's
-// own loads, the last by the scaling of the sums), or what HBM needs for the 16 KB of b that every CTA at work reads;
+// latter, measured: 0.45 to 0.47 us with 16, 32 and 64 rows of a to a tile (what a CTA's own loads take from HBM; 0.30 to 0.41
+// when b is in L2), 0.66 us with 128 (the scaling of the sums), or what HBM needs for the 16 KB of b that every CTA at work reads;
 // 0.60 us for a CTA pair on 256 x 256, 1.0 us where b has a scale a row.  Both sides of each border (us):
 // 64 x 4096 x 4096 split 1 / 2 / 4 / 8: 16.8 / 12.1 / 9.4 / 19.0; 1 x 8192 x 8192 (weights from HBM): 28.1 / 20.2 / 18.3 / 20.5,
 // 1 x 28672 x 8192: 42.9 / 49.8 / 56.0 / 61.5; 128 x 4096 x 4096
@@ -682,7 +685,7 @@ namespace mxq {
 struct Fp8Plan { int nt, split; };                 // nt 0: CTA pairs
 static Fp8Plan plan_fp8(int64_t M, int64_t N, int64_t blocks, bool b_rows, bool tma_out) {
     const double sms = sm_count(), fixed = 4.5, hbm = 5.5e6;       // us, bytes a us
-    const double block_us[4] = {0.30, 0.36, 0.41, 0.66};
+    const double block_us[4] = {0.45, 0.47, 0.47, 0.66};
     Fp8Plan best = {16, 1};
     double best_us = 1e300;
     for (int i = 0; i < 4; ++i) {

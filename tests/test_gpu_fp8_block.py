@@ -185,3 +185,40 @@ def test_repeats_exactly_on_other_streams_and_in_graphs(mx):
     for _ in range(3):
         g.replay()
     assert torch.equal(y, mx.fp8_block_linear(x2, q, b))
+
+
+def test_linear_mixed_types_one_dimension_and_views(mx):
+    x, w, b = values(6, 260, BF16, 21), values(260, 90, F32, 22, 0.05), values(1, 90, F32, 23)[0]
+    xd, wd, bd = x.cuda().requires_grad_(), w.cuda().t().requires_grad_(), b.cuda().requires_grad_()      # a transposed view as weight
+    dy = values(6, 90, BF16, 24)
+    y = mx.fp8_block_linear(xd, wd, bd)
+    got = (y, *torch.autograd.grad(y, (xd, wd, bd), dy.cuda()))
+    xv, wv = ref.quantize(x, "fp8_e4m3")[2], ref.quantize(w.t(), "fp8_e4m3", True)[2]
+    dyv, dytv, xtv = (ref.quantize(v, "fp8_e4m3")[2] for v in (dy, dy.t(), x.t()))
+    for t, (want, room), dt in ((got[0], ref.product_bound(xv, wv, BF16, b), BF16), (got[1], ref.product_bound(dyv, wv.t(), BF16), BF16),
+                                (got[2], ref.product_bound(dytv, xtv, F32), F32)):
+        assert t.dtype == dt and bool(((t.detach().cpu().double() - want).abs() <= room).all())
+    assert got[3].dtype == F32
+    one = mx.fp8_block_linear(xd.detach()[3], wd.detach(), bd.detach())
+    assert one.shape == (90,) and torch.equal(one, y.detach()[3])
+    leaf = xd.detach()[3].clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(mx.fp8_block_linear(leaf, wd.detach(), bd.detach()), leaf, dy.cuda()[3])[0], got[1][3])
+
+
+def test_prefix_of_a_larger_buffer_is_left_alone_behind_its_end(mx):
+    """The product writes [M, N] and nothing behind it; the operands' padding is not read as values."""
+    from microxcaling_b200 import _backend
+    for M, N, K in ((3, 130, 100), (300, 1000, 130), (2050, 2311, 200)):
+        a, b = (mx.quantize_fp8_block(values(r, K, BF16, r).cuda(), tile=t) for r, t in ((M, False), (N, True)))
+        want = mx.fp8_block_matmul(a, b)
+        dirty = []
+        for o in (a, b):                                       # other bytes in the padding between rows
+            pitch = o.codes.stride(0) if o.codes.shape[0] > 1 else (K + 15) // 16 * 16
+            buf = torch.full((o.codes.shape[0], pitch), 0x7f, dtype=torch.uint8, device="cuda")
+            buf[:, :K] = o.codes.view(torch.uint8) if o.codes.is_contiguous() else o.codes.contiguous().view(torch.uint8)
+            dirty.append(mx.BlockFP8(buf.view(torch.float8_e4m3fn)[:, :K], o.scales))
+        out = torch.full((M * N + 64,), 7.0, dtype=BF16, device="cuda")
+        L = _backend.lib()
+        p = [(o.codes.data_ptr(), _backend._pitch(o.codes), o.scales.data_ptr(), int(o.tile), 0) for o in dirty]
+        _backend.check(L.mxq_fp8_gemm(*p[0], *p[1], out.data_ptr(), 2, None, 0, M, N, K, _backend._stream(out)))
+        assert torch.equal(out[:M * N].view(M, N), want) and bool((out[M * N:] == 7).all())
