@@ -588,34 +588,36 @@ static int launch_norm(const NormArgs& g, bool bwd, cudaStream_t st) {
 template <int DT, int WDT, int VEC>
 static int launch_norm_vec(const NormArgs& g, bool bwd, cudaStream_t st) {
     const NormShape s = norm_shape(g.cols);
-    if constexpr (VEC > 1) {
-        if (!bwd && g.cols > 512 && g.rows >= 4 * sm_count()) {
-            if (g.cols <= 1024) return launch_norm_fwd<DT, WDT, VEC, 32, 32>(g, st);
-            // few barriers and many rows in flight: 32 or, packed two to a register, 64 values a thread.  16384 x 8192 bf16:
-            // 512 threads x 16 values 143 us, 256 x 32 107 us, 128 x 64 92 us; 65536 x 2048: 128 x 16 108, 64 x 32 89
-            if (g.cols <= 2048) return launch_norm_fwd<DT, WDT, VEC, 64, 32>(g, st);
-            if constexpr (DT == DT_F32) {
-                if (g.cols <= 4096) return launch_norm_fwd<DT, WDT, VEC, 128, 32>(g, st);
-                return launch_norm_fwd<DT, WDT, VEC, 256, 32>(g, st);
-            } else {
-                if (g.cols <= 4096) return launch_norm_fwd<DT, WDT, VEC, 64, 64>(g, st);
-                return launch_norm_fwd<DT, WDT, VEC, 128, 64>(g, st);
-            }
-        }
-        if (bwd && s.tpr > 32) {                               // whole vectors and 16-byte aligned rows
-
-            if (s.tpr == 128 && s.vals == 8) return launch_ring<DT, WDT, 128, 8>(g, st);
-            if (s.tpr == 128) return launch_ring<DT, WDT, 128, 16>(g, st);
-            if (s.tpr == 256) return launch_ring<DT, WDT, 256, 16>(g, st);
-            return launch_ring<DT, WDT, 512, 16>(g, st);
-        }
-    }
     if (s.tpr == 32 && s.vals == 8) return launch_norm<DT, WDT, VEC, 32, 8>(g, bwd, st);
     if (s.tpr == 32) return launch_norm<DT, WDT, VEC, 32, 16>(g, bwd, st);
-    if (s.tpr == 128 && s.vals == 8) return launch_norm<DT, WDT, VEC, 128, 8>(g, bwd, st);
-    if (s.tpr == 128) return launch_norm<DT, WDT, VEC, 128, 16>(g, bwd, st);
-    if (s.tpr == 256) return launch_norm<DT, WDT, VEC, 256, 16>(g, bwd, st);
-    return launch_norm<DT, WDT, VEC, 512, 16>(g, bwd, st);
+    if constexpr (VEC == 1) {
+        if (s.tpr == 128 && s.vals == 8) return launch_norm<DT, WDT, VEC, 128, 8>(g, bwd, st);
+        if (s.tpr == 128) return launch_norm<DT, WDT, VEC, 128, 16>(g, bwd, st);
+        if (s.tpr == 256) return launch_norm<DT, WDT, VEC, 256, 16>(g, bwd, st);
+        return launch_norm<DT, WDT, VEC, 512, 16>(g, bwd, st);
+    } else if (bwd) {                                          // whole vectors and 16-byte aligned rows
+        if (s.tpr == 128 && s.vals == 8) return launch_ring<DT, WDT, 128, 8>(g, st);
+        if (s.tpr == 128) return launch_ring<DT, WDT, 128, 16>(g, st);
+        if (s.tpr == 256) return launch_ring<DT, WDT, 256, 16>(g, st);
+        return launch_ring<DT, WDT, 512, 16>(g, st);
+    } else if (g.rows >= 4 * sm_count()) {
+        // few barriers and many rows in flight: 32 or, packed two to a register, 64 values a thread.  16384 x 8192 bf16:
+        // 512 threads x 16 values 143 us, 256 x 32 107 us, 128 x 64 92 us; 65536 x 2048: 128 x 16 108, 64 x 32 89
+        if (g.cols <= 1024) return launch_norm_fwd<DT, WDT, VEC, 32, 32>(g, st);
+        if (g.cols <= 2048) return launch_norm_fwd<DT, WDT, VEC, 64, 32>(g, st);
+        if constexpr (DT == DT_F32) {
+            if (g.cols <= 4096) return launch_norm_fwd<DT, WDT, VEC, 128, 32>(g, st);
+            return launch_norm_fwd<DT, WDT, VEC, 256, 32>(g, st);
+        } else {
+            if (g.cols <= 4096) return launch_norm_fwd<DT, WDT, VEC, 64, 64>(g, st);
+            return launch_norm_fwd<DT, WDT, VEC, 128, 64>(g, st);
+        }
+    } else {                                                   // few rows: many threads on each
+        if (s.tpr == 128 && s.vals == 8) return launch_norm_fwd<DT, WDT, VEC, 128, 8>(g, st);
+        if (s.tpr == 128) return launch_norm_fwd<DT, WDT, VEC, 128, 16>(g, st);
+        if (s.tpr == 256) return launch_norm_fwd<DT, WDT, VEC, 256, 16>(g, st);
+        return launch_norm_fwd<DT, WDT, VEC, 512, 16>(g, st);
+    }
 }
 
 template <int DT, int WDT>

@@ -38,6 +38,17 @@ def test_forward_and_gradients(mx, cols, dtypes):
             ref.check(t, pair)
 
 
+@pytest.mark.parametrize("cols", [16, 264, 520, 1024, 1032, 2048, 2056, 4096, 4104, 8192, 9008])
+@pytest.mark.parametrize("dtypes", [(BF16, BF16), (F16, F32), (F32, F32)])
+def test_many_rows(mx, cols, dtypes):
+    """More rows than four on an SM: other shapes of the forward kernel, and every ring of the gradient's wraps around."""
+    x, w, b, dy = inputs(1300 if cols <= 4104 else 700, cols, *dtypes, seed=cols)
+    leaves = [t.cuda().requires_grad_() for t in (x, w, b)]
+    y = mx.fused_layer_norm(*leaves)
+    for t, pair in zip((y, *torch.autograd.grad(y, leaves, dy.cuda())), ref.layer_norm(x, w, b, 1e-5, dy)):
+        ref.check(t, pair)
+
+
 @pytest.mark.parametrize("cols", [24, 129, 4096, 9000])
 def test_parts_and_missing_weights(mx, cols):
     x, w, b, dy = inputs(40, cols, BF16, F32)

@@ -96,6 +96,25 @@ def test_values_and_gradient(mx, vocab, dtype, temperature):
     assert e.logprobs is None and torch.equal(e.entropy, r.entropy)
 
 
+@pytest.mark.parametrize("vocab", [8200, 32003])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_many_rows(mx, vocab, dtype):
+    """More rows than SMs: another number of threads a row; rows that start off every 16-byte border."""
+    x, t = logits(200, vocab, dtype, seed=7)
+    leaf = x.cuda().requires_grad_()
+    r = mx.token_logprobs(leaf, t.cuda(), top=32, entropy=True)
+    lp, H, p, e_lz, e_lp, e_H, *_ = reference(x, t)
+    assert bool(((r.logprobs.detach().cpu().double() - lp[torch.arange(200), t]).abs() <= e_lp).all())
+    assert bool(((r.entropy.detach().cpu().double() - H).abs() <= e_H).all())
+    assert torch.equal(r.top_tokens.cpu(), x.sort(dim=1, descending=True, stable=True)[1][:, :32])
+    g, = torch.autograd.grad(r.logprobs.sum(), leaf)
+    want = -p
+    want[torch.arange(200), t] += 1
+    # 2^-18: log p is at most 40 in magnitude, its exponent and log z are off by a few 2^-22 of that
+    room = p * 2.0 ** -18 + want.abs() * (torch.finfo(dtype).eps / 2 + 2.0 ** -22) + 2.0 ** -40
+    assert bool(((g.cpu().double() - want).abs() <= room).all())
+
+
 def test_gradient_against_differences(mx):
     """d lp / d x_j by central differences of the 64-bit function."""
     x, t = logits(3, 50, F32, seed=5, barred=0)
