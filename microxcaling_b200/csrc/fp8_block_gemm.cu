@@ -291,7 +291,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
 // 1.4 GHz under the power cap); with B_ROWS 4096 x 4096 x 8192 259 us (1.06 PFLOP/s; 281 us when every thread held one row and
 // read all column scales).  With the scaling left out the same loop takes 119 us and 2.7 ms: the rest is the hand-over of the accumulators
 // (two of them, a round trip of a block's MMAs, drain and arrival each), not the arithmetic.  Tried and dropped: a release
-// fence at that hand-over (299 instead of 181 us at that stage), halves of an accumulator handed over apart (194 to 177).
+// fence at that hand-over (299 instead of 181 us at that stage), halves of an accumulator handed over apart (194 to 177), the
+// block loop unrolled twice (3.5 -> 4.0 ms at the large size), column scales kept in registers across rows (259 -> 325 us: spills).
 // ---------------------------------------------------------------------------------------------------------------
 struct Fp8Pair {
     const float* sa;
